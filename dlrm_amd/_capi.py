@@ -22,7 +22,7 @@ class DlrmError(RuntimeError):
     pass
 
 
-ABI_VERSION = 1018   # DLRM_ABI_VERSION of include/dlrm_amd.h these structures mirror
+ABI_VERSION = 1019   # DLRM_ABI_VERSION of include/dlrm_amd.h these structures mirror
 
 
 class EmbBagDesc(C.Structure):
@@ -55,6 +55,13 @@ class SparseOpt(C.Structure):
     ]
 
 
+class Act8Desc(C.Structure):
+    _fields_ = [
+        ("d_codes", C.c_void_p), ("ld", C.c_int64),
+        ("d_exps", C.c_void_p), ("exps_ld", C.c_int64),
+    ]
+
+
 class LinearDesc(C.Structure):
     _fields_ = [
         ("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32),
@@ -82,6 +89,35 @@ class LinearBwdDesc(C.Structure):
         ("gemm_mode", C.c_int32),
         ("d_dz_absmax", C.c_void_p), ("d_w_absmax", C.c_void_p), ("d_x_absmax", C.c_void_p), ("d_dx_absmax", C.c_void_p),
         ("w_planes", C.c_void_p),
+        ("x8", Act8Desc), ("relu_mask8", Act8Desc),
+    ]
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = [
+        ("M", C.c_int64), ("N", C.c_int32), ("dtype", C.c_int32),
+        ("d_x", C.c_void_p), ("x_ld", C.c_int64),
+        ("d_gamma", C.c_void_p), ("d_beta", C.c_void_p),
+        ("d_y", C.c_void_p), ("y_ld", C.c_int64),
+        ("d_mean", C.c_void_p), ("d_rstd", C.c_void_p),
+        ("xhat8", Act8Desc), ("y8", Act8Desc),
+        ("d_y_absmax", C.c_void_p),
+        ("eps", C.c_float), ("act", C.c_int32),
+    ]
+
+
+class LayerNormBwdDesc(C.Structure):
+    _fields_ = [
+        ("M", C.c_int64), ("N", C.c_int32), ("dtype", C.c_int32),
+        ("d_x", C.c_void_p), ("x_ld", C.c_int64),
+        ("xhat8", Act8Desc),
+        ("d_mean", C.c_void_p), ("d_rstd", C.c_void_p), ("d_gamma", C.c_void_p),
+        ("d_dy", C.c_void_p), ("dy_ld", C.c_int64),
+        ("d_relu_mask", C.c_void_p), ("relu_mask_ld", C.c_int64),
+        ("relu_mask8", Act8Desc),
+        ("d_dx", C.c_void_p), ("dx_ld", C.c_int64),
+        ("d_dgamma", C.c_void_p), ("d_dbeta", C.c_void_p),
+        ("d_dx_absmax", C.c_void_p),
     ]
 
 

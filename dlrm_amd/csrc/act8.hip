@@ -1,0 +1,153 @@
+// Activations into 8-bit checkpoints and back (format and rounding: act8.h).
+//
+// Both directions are one pass bound by memory: float32 in or out 4 bytes an element, the checkpoint 1 1/32.  A row is
+// shared by the smallest power of two of lanes that covers it (at most a wave) and every lane moves 16 bytes of the
+// activation per step, so the 32 columns of a block sit in 8 (float32) or 4 (bf16) neighbouring lanes and its largest
+// magnitude is three (two) exchanges on the vector unit's own lane paths.
+#include "act8.h"
+
+namespace dlrm {
+
+int act8_check(const dlrm_act8 *a, int cols, const char *what) {
+    DLRM_REQUIRE(a->d_codes != nullptr && a->d_exps != nullptr, "%s: NULL codes or exponents", what);
+    const int64_t blocks = act8_blocks(cols);
+    DLRM_REQUIRE(reinterpret_cast<uintptr_t>(a->d_codes) % 16 == 0 && a->ld % 16 == 0,
+                 "%s: code rows must start on 16-byte boundaries (leading dimension %lld)", what, (long long)a->ld);
+    DLRM_REQUIRE(a->ld >= blocks * kAct8Block && a->exps_ld >= blocks,
+                 "%s: leading dimensions %lld (codes) and %lld (exponents) are too small for %d columns", what, (long long)a->ld,
+                 (long long)a->exps_ld, cols);
+    return DLRM_OK;
+}
+
+struct Act8Pass {
+    const void *src;
+    void *dst;
+    int64_t ld;            // of the activation
+    int8_t *codes;
+    int64_t codes_ld;
+    uint8_t *exps;
+    int64_t exps_ld;
+    int64_t rows;
+    int cols, blocks;
+    int lanes_log2;        // lanes that share a row: 2^lanes_log2, a wave at most
+};
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void act8_pack_kernel(Act8Pass p) {
+    const int lane = threadIdx.x & 63, lanes = 1 << p.lanes_log2;
+    const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC, width = p.blocks * kAct8Block;
+    const int rows_per_wave = 64 >> p.lanes_log2;
+    const int64_t n_waves = (int64_t)gridDim.x * 4;
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave; r0 < p.rows; r0 += n_waves * rows_per_wave) {
+        const int64_t mine = r0 + (lane >> p.lanes_log2);
+        const bool live = mine < p.rows;
+        const int64_t r = live ? mine : p.rows - 1;
+        const T *row = static_cast<const T *>(p.src) + r * p.ld;
+        int8_t *codes = p.codes + r * p.codes_ld;
+        uint8_t *exps = p.exps + r * p.exps_ld;
+        // (every lane of the wave takes every turn: the exchanges inside act8_store need the neighbours)
+        for (int base = 0; base < width; base += 4 * step) {
+            float v[4][VEC];
+#pragma unroll
+            for (int u = 0; u < 4; u++) load_elems<T, VEC>(row, base + u * step + first, p.cols, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (base + u * step < width) act8_store<VEC>(v[u], codes, exps, base + u * step + first, p.blocks, live);
+        }
+    }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void act8_unpack_kernel(Act8Pass p) {
+    const int lane = threadIdx.x & 63, lanes = 1 << p.lanes_log2;
+    const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC;
+    const int rows_per_wave = 64 >> p.lanes_log2;
+    const int64_t n_waves = (int64_t)gridDim.x * 4;
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave; r0 < p.rows; r0 += n_waves * rows_per_wave) {
+        const int64_t r = r0 + (lane >> p.lanes_log2);
+        if (r >= p.rows) continue;
+        T *row = static_cast<T *>(p.dst) + r * p.ld;
+        const int8_t *codes = p.codes + r * p.codes_ld;
+        const uint8_t *exps = p.exps + r * p.exps_ld;
+        for (int c0 = first; c0 < p.cols; c0 += 4 * step) {
+            unsigned w[4][VEC == 8 ? 2 : 1];
+            int e[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int c = c0 + u * step;
+                act8_load<VEC>(codes, c, p.blocks, w[u]);
+                e[u] = c < p.cols ? exps[c / kAct8Block] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int c = c0 + u * step;
+                float v[VEC];
+                act8_values<VEC>(w[u], act8_step(e[u]), v);
+                if (c < p.cols) store_elems<T, VEC>(row, c, p.cols, v);
+            }
+        }
+    }
+}
+
+// lanes per row and workgroups: at least a wave's worth of steps per row is not needed, so narrow rows share a wave
+static unsigned act8_grid(Act8Pass &p, int vec) {
+    const int per_row = (int)ceil_div((int64_t)p.blocks * kAct8Block, vec);
+    p.lanes_log2 = vec == 1 ? 5 : 3;       // a block's lanes stay together
+    while (p.lanes_log2 < 6 && (1 << p.lanes_log2) < per_row) p.lanes_log2++;
+    const int64_t want = ceil_div(p.rows, (int64_t)4 * (64 >> p.lanes_log2));
+    return (unsigned)(want < 4096 ? want : 4096);
+}
+
+static int act8_args(const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld, const dlrm_act8 *a) {
+    DLRM_REQUIRE(a != nullptr, "checkpoint descriptor is NULL");
+    DLRM_REQUIRE(dtype == DLRM_F32 || dtype == DLRM_BF16, "dtype %d is neither DLRM_F32 nor DLRM_BF16", dtype);
+    DLRM_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 30) && x_ld >= cols, "bad shape: %lld rows of %d columns, leading dimension %lld",
+                 (long long)rows, cols, (long long)x_ld);
+    DLRM_REQUIRE(rows == 0 || d_x != nullptr, "NULL activation");
+    DLRM_REQUIRE(reinterpret_cast<uintptr_t>(d_x) % (dtype == DLRM_F32 ? 4 : 2) == 0, "activation is not aligned to its elements");
+    return rows == 0 ? DLRM_OK : act8_check(a, cols, "checkpoint");
+}
+
+static Act8Pass act8_pass(const dlrm_act8 *a, int64_t rows, int cols, int64_t x_ld) {
+    Act8Pass p{};
+    p.ld = x_ld; p.codes = a->d_codes; p.codes_ld = a->ld; p.exps = a->d_exps; p.exps_ld = a->exps_ld;
+    p.rows = rows; p.cols = cols; p.blocks = act8_blocks(cols);
+    return p;
+}
+
+}  // namespace dlrm
+
+using namespace dlrm;
+
+#define DLRM_ACT8_LAUNCH(KERNEL)                                                                                              \
+    do {                                                                                                                      \
+        const int size = dtype == DLRM_F32 ? 4 : 2;                                                                           \
+        const bool wide = reinterpret_cast<uintptr_t>(d_x) % 16 == 0 && x_ld * size % 16 == 0;                                  \
+        const unsigned grid = act8_grid(p, wide ? 16 / size : 1);                                                             \
+        hipStream_t s = as_stream(stream);                                                                                    \
+        if (dtype == DLRM_F32 && wide) hipLaunchKernelGGL((KERNEL<float, 4>), dim3(grid), dim3(256), 0, s, p);                  \
+        else if (dtype == DLRM_F32) hipLaunchKernelGGL((KERNEL<float, 1>), dim3(grid), dim3(256), 0, s, p);                     \
+        else if (wide) hipLaunchKernelGGL((KERNEL<uint16_t, 8>), dim3(grid), dim3(256), 0, s, p);                               \
+        else hipLaunchKernelGGL((KERNEL<uint16_t, 1>), dim3(grid), dim3(256), 0, s, p);                                         \
+        DLRM_LAUNCH_CHECK();                                                                                                  \
+    } while (0)
+
+extern "C" int dlrm_act8_pack(const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld, const dlrm_act8 *out,
+                              dlrm_stream_t stream) {
+    if (int rc = act8_args(d_x, dtype, rows, cols, x_ld, out)) return rc;
+    if (rows == 0) return DLRM_OK;
+    Act8Pass p = act8_pass(out, rows, cols, x_ld);
+    p.src = d_x;
+    DLRM_ACT8_LAUNCH(act8_pack_kernel);
+    return DLRM_OK;
+}
+
+extern "C" int dlrm_act8_unpack(const dlrm_act8 *a, int64_t rows, int32_t cols, void *d_x, int32_t dtype, int64_t x_ld,
+                                dlrm_stream_t stream) {
+    if (int rc = act8_args(d_x, dtype, rows, cols, x_ld, a)) return rc;
+    if (rows == 0) return DLRM_OK;
+    Act8Pass p = act8_pass(a, rows, cols, x_ld);
+    p.dst = d_x;
+    DLRM_ACT8_LAUNCH(act8_unpack_kernel);
+    return DLRM_OK;
+}

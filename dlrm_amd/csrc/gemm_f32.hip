@@ -38,6 +38,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "act8.h"
 #include "common.h"
 #include "skinny.h"
 
@@ -64,6 +65,8 @@ struct GemmParams {
     int relu;             // max(.,0) after the bias
     const float *mask;    // [M,N] (ld mask_ld) or NULL: C = (mask > 0) ? C : 0
     int64_t mask_ld;
+    const int8_t *mask8;  // or NULL: the codes of an 8-bit checkpoint in the mask's place (rows on 16-byte boundaries)
+    int64_t mask8_ld;
     int a_vec, b_vec;     // operand rows are 16-byte aligned: 16-byte global loads allowed
     int gx, gy, gz;       // logical grid: column tiles, row tiles, reduction splits
     int k_per_split;      // reduction elements per split (multiple of BK)
@@ -75,6 +78,16 @@ struct GemmParams {
     const unsigned char *bp_h, *bp_l;   // gemm_f16p_kernel: the f16 planes of B, [reduction step][N rounded up to 256][32] f16,
     int64_t bp_ld;                      // zero padded; bp_ld = bytes per reduction step
 };
+
+// four mask elements of row m from column cn on (cn a multiple of 4), as numbers whose sign decides
+__device__ inline float4 mask4(const GemmParams &p, int64_t m, int cn) {
+    if (p.mask8 == nullptr) return *reinterpret_cast<const float4 *>(p.mask + m * p.mask_ld + cn);
+    const unsigned w = *reinterpret_cast<const unsigned *>(p.mask8 + m * p.mask8_ld + cn);
+    return make_float4(act8_positive(w & 0xff), act8_positive((w >> 8) & 0xff), act8_positive((w >> 16) & 0xff), act8_positive(w >> 24));
+}
+__device__ inline bool mask_lets_pass(const GemmParams &p, int64_t m, int c) {
+    return p.mask8 ? act8_positive(p.mask8[m * p.mask8_ld + c]) : p.mask[m * p.mask_ld + c] > 0.f;
+}
 
 // Global -> register staging of one operand tile (4 x 16 bytes per thread).
 // RC: tile rows are output indices, 32 reduction elements (128 B) each: 8 lanes per row.
@@ -186,12 +199,12 @@ __device__ inline void store_output(const GemmParams &p, const f32x16 (&acc)[MI]
         // the mask pieces of this row block are requested before the block is parked, so that they travel while the
         // accumulators go through LDS (one round trip to memory per block instead of one per group of rows)
         float4 mk[32 / RPI];
-        const bool mask_vec = p.mask != nullptr && c_vec && cn + 3 < p.N;
+        const bool mask_vec = (p.mask != nullptr || p.mask8 != nullptr) && c_vec && cn + 3 < p.N;
         if (mask_vec) {
 #pragma unroll
             for (int it = 0; it < 32 / RPI; it++) {
                 const int m = m0 + wr * (32 * MI) + mi * 32 + it * RPI + (lane / LPR);
-                mk[it] = *reinterpret_cast<const float4 *>(p.mask + (int64_t)(m < p.M ? m : p.M - 1) * p.mask_ld + cn);
+                mk[it] = mask4(p, m < p.M ? m : p.M - 1, cn);
             }
         }
 #pragma unroll
@@ -224,7 +237,7 @@ __device__ inline void store_output(const GemmParams &p, const f32x16 (&acc)[MI]
                 for (int q = 0; q < 4; q++)
                     if (cn + q < p.N) {
                         float x = e[q];
-                        if (p.mask) x = p.mask[(int64_t)m * p.mask_ld + cn + q] > 0.f ? x : 0.f;
+                        if (p.mask || p.mask8) x = mask_lets_pass(p, m, cn + q) ? x : 0.f;
                         dst[q] = x;
                         vmax = fmaxf(vmax, fabsf(x));
                     }
@@ -1180,12 +1193,12 @@ __device__ inline void store_output16(const GemmParams &p, const f32x4 (&acc)[2]
         if (cn + 3 < p.N) bv.w = p.bias[cn + 3];
     }
     float4 mk[32 / RPI];
-    const bool mask_vec = p.mask != nullptr && c_vec && cn + 3 < p.N;
+    const bool mask_vec = (p.mask != nullptr || p.mask8 != nullptr) && c_vec && cn + 3 < p.N;
     if (mask_vec) {
 #pragma unroll
         for (int it = 0; it < 32 / RPI; it++) {
             const int m = m0 + wave * 32 + it * RPI + (lane / LPR);
-            mk[it] = *reinterpret_cast<const float4 *>(p.mask + (int64_t)(m < p.M ? m : p.M - 1) * p.mask_ld + cn);
+            mk[it] = mask4(p, m < p.M ? m : p.M - 1, cn);
         }
     }
 #pragma unroll
@@ -1219,7 +1232,7 @@ __device__ inline void store_output16(const GemmParams &p, const f32x4 (&acc)[2]
             for (int q = 0; q < 4; q++)
                 if (cn + q < p.N) {
                     float x = e[q];
-                    if (p.mask) x = p.mask[(int64_t)m * p.mask_ld + cn + q] > 0.f ? x : 0.f;
+                    if (p.mask || p.mask8) x = mask_lets_pass(p, m, cn + q) ? x : 0.f;
                     dst[q] = x;
                     vmax = fmaxf(vmax, fabsf(x));
                 }
@@ -1916,14 +1929,19 @@ extern "C" int dlrm_linear_backward_data(const dlrm_linear_bwd *l, dlrm_stream_t
     DLRM_REQUIRE(l->M < (1ll << 31), "M too large");
     DLRM_REQUIRE(l->d_dz && l->d_w && l->d_dx, "NULL operand");
     DLRM_REQUIRE(l->dz_ld >= l->N && l->w_ld >= l->K && l->dx_ld >= l->K, "leading dimension too small");
+    if (l->relu_mask8.d_codes) {
+        DLRM_REQUIRE(l->d_relu_mask == nullptr, "two ReLU masks given");
+        if (int rc = act8_check(&l->relu_mask8, l->K, "checkpoint of the ReLU output")) return rc;
+    }
     if (l->N == 1 && gemv_ok(l->d_dx, l->dx_ld, l->d_w, l->K) &&
         (l->d_relu_mask == nullptr || gemv_ok(l->d_relu_mask, l->relu_mask_ld, l->d_w, l->K)))
-        return gemv_backward_data(l->d_dz, l->dz_ld, l->d_w, l->d_dx, l->dx_ld, l->d_relu_mask, l->relu_mask_ld, (int)l->M,
-                                  l->K, l->d_dx_absmax, as_stream(stream));
+        return gemv_backward_data(l->d_dz, l->dz_ld, l->d_w, l->d_dx, l->dx_ld, l->d_relu_mask, l->relu_mask_ld,
+                                  l->relu_mask8.d_codes, l->relu_mask8.ld, (int)l->M, l->K, l->d_dx_absmax, as_stream(stream));
     GemmParams p{};
     p.A = l->d_dz; p.lda = l->dz_ld; p.B = l->d_w; p.ldb = l->w_ld; p.C = l->d_dx; p.ldc = l->dx_ld;
     p.M = (int)l->M; p.N = l->K; p.K = l->N;  // C = dx [M,K], reduction over N
     p.mask = l->d_relu_mask; p.mask_ld = l->relu_mask_ld;
+    p.mask8 = l->relu_mask8.d_codes; p.mask8_ld = l->relu_mask8.ld;
     p.a_vec = vec_ok(p.A, p.lda); p.b_vec = vec_ok(p.B, p.ldb);
     p.k_per_split = (int)ceil_div(l->N, BK) * BK;
     p.c_max = l->d_dx_absmax;
@@ -1961,8 +1979,12 @@ static int backward_weight_impl(const dlrm_linear_bwd *l, void *d_workspace, siz
     DLRM_REQUIRE(l != nullptr, "linear_bwd descriptor is NULL");
     DLRM_REQUIRE(l->M >= 1 && l->N >= 1 && l->K >= 1, "bad shape");
     DLRM_REQUIRE(l->M < (1ll << 31), "M too large");
-    DLRM_REQUIRE(l->d_dz && l->d_x && l->d_dw, "NULL operand");
-    DLRM_REQUIRE(l->dz_ld >= l->N && l->x_ld >= l->K && l->dw_ld >= l->K, "leading dimension too small");
+    const bool from8 = l->x8.d_codes != nullptr;
+    DLRM_REQUIRE(l->d_dz && (l->d_x || from8) && l->d_dw, "NULL operand");
+    DLRM_REQUIRE(!from8 || l->d_x == nullptr, "both x and its 8-bit checkpoint given");
+    DLRM_REQUIRE(l->dz_ld >= l->N && (from8 || l->x_ld >= l->K) && l->dw_ld >= l->K, "leading dimension too small");
+    if (from8)
+        if (int rc = act8_check(&l->x8, l->K, "checkpoint of x")) return rc;
     size_t need = 0;
     dlrm_linear_backward_weight_workspace_bytes(l->M, l->N, l->K, &need);
     DLRM_REQUIRE(d_workspace != nullptr && workspace_bytes >= need, "workspace too small: %zu < %zu", workspace_bytes,
@@ -1970,8 +1992,23 @@ static int backward_weight_impl(const dlrm_linear_bwd *l, void *d_workspace, siz
     DLRM_REQUIRE(aligned16(d_workspace), "workspace must be 16-byte aligned");
     hipStream_t s = as_stream(stream);
     int splits = 1;
-    const TileShape ts = wgrad_shape(l->M, l->N, l->K, l->gemm_mode, &splits);
+    const TileShape ts = wgrad_shape(l->M, l->N, l->K, from8 ? DLRM_GEMM_BF16X3 : l->gemm_mode, &splits);
     float *slabs = static_cast<float *>(d_workspace);
+    if (from8) {
+        Wgrad8 w{};
+        w.dz = l->d_dz; w.dz_ld = l->dz_ld; w.dz_vec = vec_ok(l->d_dz, l->dz_ld);
+        w.codes = l->x8.d_codes; w.codes_ld = l->x8.ld; w.exps = l->x8.d_exps; w.exps_ld = l->x8.exps_ld;
+        w.blocks = act8_blocks(l->K);
+        w.M = (int)l->M; w.N = l->N; w.K = l->K;
+        w.rows_per_split = (int)ceil_div(ceil_div(l->M, splits), BK) * BK;
+        w.gz = (int)ceil_div(l->M, w.rows_per_split);
+        float *db_slabs = slabs + (size_t)splits * l->N * l->K;
+        const bool whole = w.gz == 1;
+        w.C = whole ? l->d_dw : slabs; w.ldc = whole ? l->dw_ld : l->K; w.slab_stride = (int64_t)l->N * l->K;
+        w.colsum = l->d_db == nullptr ? nullptr : (whole ? l->d_db : db_slabs);
+        if (int rc = launch_wgrad8(w, ts.tm, ts.tn, s)) return rc;
+        return whole ? DLRM_OK : launch_reduce(slabs, w.slab_stride, l->N, l->K, l->d_dw, l->dw_ld, db_slabs, l->d_db, w.gz, s, pending);
+    }
     const bool few_inputs = skinny_k_forward_ok(l->N, l->K);
     if (few_inputs || (l->N == 1 && gemv_backward_weight_ok(l->d_x, l->x_ld, l->K))) {
         // partial sums over row ranges, then the same fixed-order reduction as the split-batch product

@@ -1,0 +1,626 @@
+// Layer norm over the rows of an activation, forward and backward.
+//
+//   forward    mean = sum x / N, rstd = 1 / sqrt(sum (x - mean)^2 / N + eps), xh = (x - mean) rstd, y = act(gamma xh + beta)
+//   backward   d = dy where the ReLU let y through, else 0;  c1 = sum gamma d / N, c2 = sum gamma d xh / N
+//              dx = rstd (gamma d - c1 - xh c2),  dgamma = sum over rows of d xh,  dbeta = sum over rows of d
+//
+// Both are bound by memory, so a row is read once: a team of lanes holds it in registers between the sums and the output
+// (8 to 64 lanes of a wave for rows up to 2048, a workgroup of 256 or 1024 threads up to 16384).  Deviations are squared
+// after the mean is known, not as sum x^2 - N mean^2, which loses everything when the mean is large.  Statistics and
+// sums are float32 whatever the activation's type.  Longer rows are read again for every sum (the *_long kernels).
+//
+// The backward kernel's teams walk over many rows and keep their columns' share of dgamma and dbeta in registers; a
+// workgroup leaves one partial row of each in the workspace and param_sums_kernel adds those in a fixed order: no
+// atomics, the same bits every time.
+#include "act8.h"
+
+namespace dlrm {
+
+constexpr int kLongRow = 16384;      // longest row that stays in registers
+
+struct NormFwd {
+    const void *x;
+    int64_t x_ld;
+    const float *gamma, *beta;
+    void *y;
+    int64_t y_ld;
+    float *mean, *rstd;
+    dlrm_act8 xhat8, y8;
+    float *y_max;
+    int64_t M;
+    int N;
+    float eps;
+    int relu;
+};
+
+struct NormBwd {
+    const void *x;              // or NULL: xhat8
+    int64_t x_ld;
+    dlrm_act8 xhat8;
+    const float *mean, *rstd, *gamma;
+    const void *dy;
+    int64_t dy_ld;
+    const void *mask;           // y of the forward pass, or NULL
+    int64_t mask_ld;
+    dlrm_act8 mask8;
+    void *dx;
+    int64_t dx_ld;
+    float *part_g, *part_b;     // [workgroups][part_stride] partial sums, or NULL
+    int64_t part_stride;
+    float *dx_max;
+    int64_t M;
+    int N;
+};
+
+// sum over the TEAM lanes that share a row, the same bits in all of them.  Teams of several waves meet in `slot` (TEAM / 64
+// floats): the caller alternates between slots, so that a slot is written again only behind a later barrier.
+template <int TEAM>
+__device__ inline float team_sum(float x, float *slot) {
+    if constexpr (TEAM <= 64) return group_sum<TEAM>(x);
+    else {
+        x = group_sum<64>(x);
+        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+        __syncthreads();
+        float t = slot[0];
+#pragma unroll
+        for (int w = 1; w < TEAM / 64; w++) t += slot[w];
+        return t;
+    }
+}
+template <int TEAM>
+__device__ inline void team_sum2(float &x, float &y, float *slot) {     // slot: 2 TEAM / 64 floats
+    if constexpr (TEAM <= 64) {
+        x = group_sum<TEAM>(x);
+        y = group_sum<TEAM>(y);
+    } else {
+        constexpr int W = TEAM / 64;
+        x = group_sum<64>(x);
+        y = group_sum<64>(y);
+        if ((threadIdx.x & 63) == 0) {
+            slot[threadIdx.x >> 6] = x;
+            slot[W + (threadIdx.x >> 6)] = y;
+        }
+        __syncthreads();
+        x = slot[0];
+        y = slot[W];
+#pragma unroll
+        for (int w = 1; w < W; w++) {
+            x += slot[w];
+            y += slot[W + w];
+        }
+    }
+}
+
+__device__ inline float relu_keeping_nan(float y) { return y <= 0.f ? 0.f : y; }
+
+template <typename T, int VEC>
+__device__ inline void norm_output(const NormFwd &p, int64_t row, int c, bool live, const float (&xh)[VEC], const float (&g)[VEC],
+                                   const float (&b)[VEC], float &vmax) {
+    if (p.xhat8.d_codes)
+        act8_store<VEC>(xh, p.xhat8.d_codes + row * p.xhat8.ld, p.xhat8.d_exps + row * p.xhat8.exps_ld, c, act8_blocks(p.N), live);
+    float y[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+        y[j] = __builtin_fmaf(xh[j], g[j], b[j]);
+        if (p.relu) y[j] = relu_keeping_nan(y[j]);
+        y[j] = c + j < p.N ? rounded_to<T>(y[j]) : 0.f;
+        vmax = fmaxf(vmax, fabsf(y[j]));
+    }
+    // (the checkpoint of the stored value, so that it equals what dlrm_act8_pack makes of y)
+    if (p.y8.d_codes)
+        act8_store<VEC>(y, p.y8.d_codes + row * p.y8.ld, p.y8.d_exps + row * p.y8.exps_ld, c, act8_blocks(p.N), live);
+    if (live) store_elems<T, VEC>(static_cast<T *>(p.y) + row * p.y_ld, c, p.N, y);
+}
+
+template <typename T, int VEC, int V, int TEAM>
+__global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(NormFwd p) {
+    constexpr int kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
+    __shared__ float slots[2][TEAM > 64 ? TEAM / 64 : 1];
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    float g[V][VEC], b[V][VEC];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int c = (v * TEAM + lane) * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            g[v][j] = p.gamma && c + j < p.N ? p.gamma[c + j] : 1.f;
+            b[v][j] = p.beta && c + j < p.N ? p.beta[c + j] : 0.f;
+        }
+    }
+    float vmax = 0.f;
+    for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < p.M; r0 += (int64_t)gridDim.x * kTeams) {
+        const bool live = r0 + team < p.M;            // (the other teams of the wave go along: exchanges need every lane)
+        const int64_t row = live ? r0 + team : p.M - 1;
+        const T *xr = static_cast<const T *>(p.x) + row * p.x_ld;
+        float x[V][VEC], s = 0.f, q = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; v++) load_elems<T, VEC>(xr, (v * TEAM + lane) * VEC, p.N, x[v]);
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) s += x[v][j];
+        const float mean = team_sum<TEAM>(s, slots[0]) / (float)p.N;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                x[v][j] = (v * TEAM + lane) * VEC + j < p.N ? x[v][j] - mean : 0.f;
+                q = __builtin_fmaf(x[v][j], x[v][j], q);
+            }
+        const float rstd = 1.f / sqrtf(team_sum<TEAM>(q, slots[1]) / (float)p.N + p.eps);
+        if (lane == 0 && live) {
+            if (p.mean) p.mean[row] = mean;
+            if (p.rstd) p.rstd[row] = rstd;
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) x[v][j] *= rstd;
+            float top = 0.f;
+            norm_output<T, VEC>(p, row, (v * TEAM + lane) * VEC, live, x[v], g[v], b[v], top);
+            vmax = fmaxf(vmax, top);
+        }
+    }
+    if (p.y_max) fold_absmax(vmax, p.y_max);
+}
+
+// rows beyond kLongRow: a workgroup of 1024 threads per row, the row read once for each sum and once for the output
+template <typename T, int VEC>
+__global__ __launch_bounds__(1024) void norm_fwd_long_kernel(NormFwd p) {
+    __shared__ float slots[2][16];
+    const int first = threadIdx.x * VEC, width = act8_blocks(p.N) * kAct8Block;
+    float vmax = 0.f;
+    for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+        const T *xr = static_cast<const T *>(p.x) + row * p.x_ld;
+        float s = 0.f, q = 0.f;
+        for (int c = first; c < p.N; c += 1024 * VEC) {
+            float x[VEC];
+            load_elems<T, VEC>(xr, c, p.N, x);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) s += x[j];
+        }
+        const float mean = team_sum<1024>(s, slots[0]) / (float)p.N;
+        for (int c = first; c < p.N; c += 1024 * VEC) {
+            float x[VEC];
+            load_elems<T, VEC>(xr, c, p.N, x);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const float d = c + j < p.N ? x[j] - mean : 0.f;
+                q = __builtin_fmaf(d, d, q);
+            }
+        }
+        const float rstd = 1.f / sqrtf(team_sum<1024>(q, slots[1]) / (float)p.N + p.eps);
+        if (threadIdx.x == 0) {
+            if (p.mean) p.mean[row] = mean;
+            if (p.rstd) p.rstd[row] = rstd;
+        }
+        // (whole waves take the last turn together: a block's lanes exchange its largest magnitude)
+        for (int base = 0; base < width; base += 1024 * VEC) {
+            const int c = base + first;
+            float x[VEC], g[VEC], b[VEC];
+            load_elems<T, VEC>(xr, c, p.N, x);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                x[j] = c + j < p.N ? (x[j] - mean) * rstd : 0.f;
+                g[j] = p.gamma && c + j < p.N ? p.gamma[c + j] : 1.f;
+                b[j] = p.beta && c + j < p.N ? p.beta[c + j] : 0.f;
+            }
+            norm_output<T, VEC>(p, row, c, true, x, g, b, vmax);
+        }
+    }
+    if (p.y_max) fold_absmax(vmax, p.y_max);
+}
+
+// xh and d of VEC elements of a row
+template <typename T, int VEC, bool FROM8, int MASK>
+__device__ inline void norm_grad_elems(const NormBwd &p, int64_t row, int c, float mean, float rstd, float (&xh)[VEC],
+                                       float (&d)[VEC]) {
+    const int blocks = act8_blocks(p.N);
+    if constexpr (FROM8) {
+        unsigned w[VEC == 8 ? 2 : 1];
+        act8_load<VEC>(p.xhat8.d_codes + row * p.xhat8.ld, c, blocks, w);
+        const int e = c < p.N ? p.xhat8.d_exps[row * p.xhat8.exps_ld + c / kAct8Block] : 0;
+        act8_values<VEC>(w, act8_step(e), xh);
+    } else {
+        load_elems<T, VEC>(static_cast<const T *>(p.x) + row * p.x_ld, c, p.N, xh, mean);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) xh[j] = (xh[j] - mean) * rstd;
+    }
+    load_elems<T, VEC>(static_cast<const T *>(p.dy) + row * p.dy_ld, c, p.N, d);
+    if constexpr (MASK == 1) {
+        float y[VEC];
+        load_elems<T, VEC>(static_cast<const T *>(p.mask) + row * p.mask_ld, c, p.N, y);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) d[j] = y[j] > 0.f ? d[j] : 0.f;
+    } else if constexpr (MASK == 2) {
+        unsigned w[VEC == 8 ? 2 : 1];
+        act8_load<VEC>(p.mask8.d_codes + row * p.mask8.ld, c, blocks, w);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) d[j] = act8_positive((w[j / 4] >> (8 * (j % 4))) & 0xff) ? d[j] : 0.f;
+    }
+}
+
+// MASK: 0 no ReLU behind the norm, 1 its output, 2 the checkpoint of its output
+template <typename T, int VEC, int V, int TEAM, bool FROM8, int MASK>
+__global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(NormBwd p) {
+    constexpr int kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
+    __shared__ float slots[2][TEAM > 64 ? TEAM / 32 : 1];
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    float g[V][VEC], acc_g[V][VEC], acc_b[V][VEC];
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        const int c = (v * TEAM + lane) * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            g[v][j] = p.gamma && c + j < p.N ? p.gamma[c + j] : 1.f;
+            acc_g[v][j] = acc_b[v][j] = 0.f;
+        }
+    }
+    float vmax = 0.f;
+    int turn = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < p.M; r0 += (int64_t)gridDim.x * kTeams, turn ^= 1) {
+        const bool live = r0 + team < p.M;
+        const int64_t row = live ? r0 + team : p.M - 1;
+        const float rstd = p.rstd[row], mean = FROM8 ? 0.f : p.mean[row];
+        float xh[V][VEC], d[V][VEC], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            norm_grad_elems<T, VEC, FROM8, MASK>(p, row, (v * TEAM + lane) * VEC, mean, rstd, xh[v], d[v]);
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                if (live) {
+                    acc_b[v][j] += d[v][j];
+                    acc_g[v][j] = __builtin_fmaf(d[v][j], xh[v][j], acc_g[v][j]);
+                }
+                d[v][j] *= g[v][j];
+                s1 += d[v][j];
+                s2 = __builtin_fmaf(d[v][j], xh[v][j], s2);
+            }
+        team_sum2<TEAM>(s1, s2, slots[turn]);
+        const float c1 = s1 / (float)p.N, c2 = s2 / (float)p.N;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int c = (v * TEAM + lane) * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                d[v][j] = rounded_to<T>(rstd * (d[v][j] - c1 - xh[v][j] * c2));
+                if (c + j < p.N) vmax = fmaxf(vmax, fabsf(d[v][j]));
+            }
+            if (live) store_elems<T, VEC>(static_cast<T *>(p.dx) + row * p.dx_ld, c, p.N, d[v]);
+        }
+    }
+    if (p.dx_max) fold_absmax(vmax, p.dx_max);
+    if (p.part_g == nullptr && p.part_b == nullptr) return;
+    // the teams' columns, added in team order
+    if constexpr (kTeams > 1) {
+        constexpr int W = V * TEAM * VEC;
+        __shared__ float meet[kTeams * W];
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            float *part = which == 0 ? p.part_g : p.part_b;
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    meet[team * W + (v * TEAM + lane) * VEC + j] = which == 0 ? acc_g[v][j] : acc_b[v][j];
+            __syncthreads();
+            if (part)
+                for (int c = threadIdx.x; c < p.N; c += kThreads) {
+                    float t = meet[c];
+                    for (int k = 1; k < kTeams; k++) t += meet[k * W + c];
+                    part[(int64_t)blockIdx.x * p.part_stride + c] = t;
+                }
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const int c = (v * TEAM + lane) * VEC + j;
+                if (c < p.N) {
+                    if (p.part_g) p.part_g[(int64_t)blockIdx.x * p.part_stride + c] = acc_g[v][j];
+                    if (p.part_b) p.part_b[(int64_t)blockIdx.x * p.part_stride + c] = acc_b[v][j];
+                }
+            }
+    }
+}
+
+// rows beyond kLongRow.  Parameter gradients: a thread per column walks over a share of the rows (before dx is written:
+// dx may be dy's own memory) ...
+template <typename T, bool FROM8, int MASK>
+__global__ __launch_bounds__(256) void norm_bwd_long_params_kernel(NormBwd p, int64_t rows_per_part) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.N) return;
+    const int64_t begin = blockIdx.y * rows_per_part;
+    const int64_t end = begin + rows_per_part < p.M ? begin + rows_per_part : p.M;
+    float ag = 0.f, ab = 0.f;
+    for (int64_t row = begin; row < end; row++) {
+        float xh[1], d[1];
+        norm_grad_elems<T, 1, FROM8, MASK>(p, row, c, FROM8 ? 0.f : p.mean[row], p.rstd[row], xh, d);
+        ab += d[0];
+        ag = __builtin_fmaf(d[0], xh[0], ag);
+    }
+    if (p.part_g) p.part_g[blockIdx.y * p.part_stride + c] = ag;
+    if (p.part_b) p.part_b[blockIdx.y * p.part_stride + c] = ab;
+}
+// ... and dx with a workgroup per row, which is read once for the sums and once for the output
+template <typename T, int VEC, bool FROM8, int MASK>
+__global__ __launch_bounds__(1024) void norm_bwd_long_kernel(NormBwd p) {
+    __shared__ float slots[2][32];
+    float vmax = 0.f;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x, turn ^= 1) {
+        const float rstd = p.rstd[row], mean = FROM8 ? 0.f : p.mean[row];
+        float xh[VEC], d[VEC], s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x * VEC; c < p.N; c += 1024 * VEC) {
+            norm_grad_elems<T, VEC, FROM8, MASK>(p, row, c, mean, rstd, xh, d);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const float gd = p.gamma && c + j < p.N ? d[j] * p.gamma[c + j] : d[j];
+                s1 += gd;
+                s2 = __builtin_fmaf(gd, xh[j], s2);
+            }
+        }
+        team_sum2<1024>(s1, s2, slots[turn]);
+        const float c1 = s1 / (float)p.N, c2 = s2 / (float)p.N;
+        for (int c = threadIdx.x * VEC; c < p.N; c += 1024 * VEC) {
+            norm_grad_elems<T, VEC, FROM8, MASK>(p, row, c, mean, rstd, xh, d);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const float gd = p.gamma && c + j < p.N ? d[j] * p.gamma[c + j] : d[j];
+                d[j] = rounded_to<T>(rstd * (gd - c1 - xh[j] * c2));
+                if (c + j < p.N) vmax = fmaxf(vmax, fabsf(d[j]));
+            }
+            store_elems<T, VEC>(static_cast<T *>(p.dx) + row * p.dx_ld, c, p.N, d);
+        }
+    }
+    if (p.dx_max) fold_absmax(vmax, p.dx_max);
+}
+
+// out[c] = sum over the partial rows of a column, for both gradients: a workgroup takes 32 columns, its 32 groups of 32
+// lanes every 32nd partial row, and the groups meet in LDS in a fixed order
+struct ParamSums {
+    const float *part[2];
+    float *out[2];
+    int64_t stride;
+    int parts, N;
+};
+__global__ __launch_bounds__(1024) void param_sums_kernel(ParamSums p) {
+    __shared__ float meet[32][33];
+    const int e = threadIdx.x & 31, q = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + e;
+    const float *part = p.part[blockIdx.y];
+    float *out = p.out[blockIdx.y];
+    if (out == nullptr) return;
+    float a = 0.f;
+    if (c < p.N) {
+        int k = q;
+        for (; k + 224 < p.parts; k += 256) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = part[(k + 32 * u) * p.stride + c];
+#pragma unroll
+            for (int u = 0; u < 8; u++) a += v[u];
+        }
+        for (; k < p.parts; k += 32) a += part[k * p.stride + c];
+    }
+    meet[q][e] = a;
+    __syncthreads();
+    if (q == 0 && c < p.N) {
+        for (int k = 1; k < 32; k++) a += meet[k][e];
+        out[c] = a;
+    }
+}
+
+// ---- launches.  Rows per width: a team of 8 to 64 lanes with up to 32 elements a lane, then 256 and 1024 threads.
+static int64_t norm_bwd_parts(int64_t M, int N) {       // most partial rows that a backward launch leaves
+    const int64_t cap = N <= 2048 ? 1024 : (N <= 8192 ? 512 : (N <= kLongRow ? 256 : 64));
+    return M < cap ? (M < 1 ? 1 : M) : cap;
+}
+
+template <typename T, int VEC, int V, int TEAM>
+static void launch_fwd(const NormFwd &p, hipStream_t s) {
+    constexpr int kThreads = TEAM > 256 ? TEAM : 256;
+    const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = TEAM > 256 ? 512 : 2048;
+    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
+}
+
+template <typename T, int VEC, int V, int TEAM, bool FROM8, int MASK>
+static void launch_bwd_as(const NormBwd &p, unsigned grid, hipStream_t s) {
+    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, V, TEAM, FROM8, MASK>), dim3(grid), dim3(TEAM > 256 ? TEAM : 256), 0, s, p);
+}
+template <typename T, int VEC, int V, int TEAM>
+static void launch_bwd(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
+    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM;
+    const int64_t want = ceil_div(p.M, kTeams), cap = norm_bwd_parts(p.M, p.N);
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
+    *parts = grid;
+    if (grid == 1) {            // a single workgroup's sums are the gradients
+        p.part_g = dgamma;
+        p.part_b = dbeta;
+    }
+    const int mask = p.mask8.d_codes ? 2 : (p.mask ? 1 : 0);
+    if (p.x == nullptr) {
+        if (mask == 0) launch_bwd_as<T, VEC, V, TEAM, true, 0>(p, grid, s);
+        else if (mask == 1) launch_bwd_as<T, VEC, V, TEAM, true, 1>(p, grid, s);
+        else launch_bwd_as<T, VEC, V, TEAM, true, 2>(p, grid, s);
+    } else {
+        if (mask == 0) launch_bwd_as<T, VEC, V, TEAM, false, 0>(p, grid, s);
+        else if (mask == 1) launch_bwd_as<T, VEC, V, TEAM, false, 1>(p, grid, s);
+        else launch_bwd_as<T, VEC, V, TEAM, false, 2>(p, grid, s);
+    }
+}
+
+template <typename T, int VEC, bool FROM8, int MASK>
+static void launch_bwd_long_as(const NormBwd &p, int64_t parts, hipStream_t s) {
+    if (p.part_g || p.part_b)
+        hipLaunchKernelGGL((norm_bwd_long_params_kernel<T, FROM8, MASK>), dim3((unsigned)ceil_div(p.N, 256), (unsigned)parts),
+                           dim3(256), 0, s, p, ceil_div(p.M, parts));
+    hipLaunchKernelGGL((norm_bwd_long_kernel<T, VEC, FROM8, MASK>), dim3((unsigned)(p.M < 512 ? p.M : 512)), dim3(1024), 0, s, p);
+}
+template <typename T, int VEC>
+static void launch_bwd_long(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
+    const int64_t n = ceil_div(p.M, ceil_div(p.M, norm_bwd_parts(p.M, p.N)));      // (every part has a row)
+    *parts = n;
+    if (n == 1) {
+        p.part_g = dgamma;
+        p.part_b = dbeta;
+    }
+    const int mask = p.mask8.d_codes ? 2 : (p.mask ? 1 : 0);
+    if (p.x == nullptr) {
+        if (mask == 0) launch_bwd_long_as<T, VEC, true, 0>(p, n, s);
+        else if (mask == 1) launch_bwd_long_as<T, VEC, true, 1>(p, n, s);
+        else launch_bwd_long_as<T, VEC, true, 2>(p, n, s);
+    } else {
+        if (mask == 0) launch_bwd_long_as<T, VEC, false, 0>(p, n, s);
+        else if (mask == 1) launch_bwd_long_as<T, VEC, false, 1>(p, n, s);
+        else launch_bwd_long_as<T, VEC, false, 2>(p, n, s);
+    }
+}
+
+// one team shape per width.  WIDE: 16 bytes a lane and step; else one element (rows that do not start on 16 bytes).
+#define DLRM_NORM_SHAPES(T, WIDE, N, CALL, LONG, ...)                          \
+    do {                                                                       \
+        constexpr int W = (WIDE) ? kWide<T> : 1, F = kWide<T> / 4;             \
+        if constexpr (WIDE) {                                                  \
+            if ((N) <= 8 * W) CALL<T, W, 1, 8>(__VA_ARGS__);                   \
+            else if ((N) <= 16 * W) CALL<T, W, 1, 16>(__VA_ARGS__);            \
+            else if ((N) <= 32 * W) CALL<T, W, 1, 32>(__VA_ARGS__);            \
+            else if ((N) <= 64 * W) CALL<T, W, 1, 64>(__VA_ARGS__);            \
+            else if ((N) <= 512 * F) CALL<T, W, 2, 64>(__VA_ARGS__);           \
+            else if ((N) <= 1024 * F) CALL<T, W, 4, 64>(__VA_ARGS__);          \
+            else if ((N) <= 2048) CALL<T, W, 8 / F, 64>(__VA_ARGS__);          \
+            else if ((N) <= 4096) CALL<T, W, 4 / F, 256>(__VA_ARGS__);         \
+            else if ((N) <= 8192) CALL<T, W, 8 / F, 256>(__VA_ARGS__);         \
+            else if ((N) <= kLongRow) CALL<T, W, 4 / F, 1024>(__VA_ARGS__);    \
+            else LONG<T, W>(__VA_ARGS__);                                      \
+        } else {                                                               \
+            if ((N) <= 32) CALL<T, 1, 1, 32>(__VA_ARGS__);                     \
+            else if ((N) <= 128) CALL<T, 1, 2, 64>(__VA_ARGS__);               \
+            else if ((N) <= 512) CALL<T, 1, 8, 64>(__VA_ARGS__);               \
+            else if ((N) <= 1024) CALL<T, 1, 16, 64>(__VA_ARGS__);             \
+            else if ((N) <= 4096) CALL<T, 1, 16, 256>(__VA_ARGS__);            \
+            else if ((N) <= kLongRow) CALL<T, 1, 16, 1024>(__VA_ARGS__);       \
+            else LONG<T, 1>(__VA_ARGS__);                                      \
+        }                                                                      \
+    } while (0)
+
+template <typename T, int VEC>
+static void launch_fwd_long(const NormFwd &p, hipStream_t s) {
+    hipLaunchKernelGGL((norm_fwd_long_kernel<T, VEC>), dim3((unsigned)(p.M < 512 ? p.M : 512)), dim3(1024), 0, s, p);
+}
+
+template <typename T>
+static void norm_fwd(const NormFwd &p, bool wide, hipStream_t s) {
+    if (wide) DLRM_NORM_SHAPES(T, true, p.N, launch_fwd, launch_fwd_long, p, s);
+    else DLRM_NORM_SHAPES(T, false, p.N, launch_fwd, launch_fwd_long, p, s);
+}
+template <typename T>
+static void norm_bwd(const NormBwd &p, bool wide, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
+    if (wide) DLRM_NORM_SHAPES(T, true, p.N, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
+    else DLRM_NORM_SHAPES(T, false, p.N, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
+}
+
+static bool rows_wide(const void *p, int64_t ld, int size) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0);
+}
+static bool rows_aligned(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
+static int norm_shape(int64_t M, int32_t N, int32_t dtype) {
+    DLRM_REQUIRE(M >= 0 && N >= 1 && N <= (1 << 30), "bad shape: %lld rows of %d columns", (long long)M, N);
+    DLRM_REQUIRE(dtype == DLRM_F32 || dtype == DLRM_BF16, "dtype %d is neither DLRM_F32 nor DLRM_BF16", dtype);
+    return DLRM_OK;
+}
+
+}  // namespace dlrm
+
+using namespace dlrm;
+
+extern "C" int dlrm_layer_norm_forward(const dlrm_layer_norm *l, dlrm_stream_t stream) {
+    DLRM_REQUIRE(l != nullptr, "layer_norm descriptor is NULL");
+    if (int rc = norm_shape(l->M, l->N, l->dtype)) return rc;
+    DLRM_REQUIRE(l->act == DLRM_ACT_NONE || l->act == DLRM_ACT_RELU, "act must be DLRM_ACT_NONE or DLRM_ACT_RELU, got %d", l->act);
+    DLRM_REQUIRE(l->eps >= 0.f, "eps must not be negative");
+    if (l->M == 0) return DLRM_OK;
+    const int size = l->dtype == DLRM_F32 ? 4 : 2;
+    DLRM_REQUIRE(l->d_x && l->d_y, "NULL operand");
+    DLRM_REQUIRE(l->x_ld >= l->N && l->y_ld >= l->N, "leading dimension too small");
+    DLRM_REQUIRE(rows_aligned(l->d_x, size) && rows_aligned(l->d_y, size), "operand is not aligned to its elements");
+    if (l->xhat8.d_codes)
+        if (int rc = act8_check(&l->xhat8, l->N, "checkpoint of the normalised rows")) return rc;
+    if (l->y8.d_codes)
+        if (int rc = act8_check(&l->y8, l->N, "checkpoint of the output")) return rc;
+    NormFwd p{};
+    p.x = l->d_x; p.x_ld = l->x_ld; p.gamma = l->d_gamma; p.beta = l->d_beta; p.y = l->d_y; p.y_ld = l->y_ld;
+    p.mean = l->d_mean; p.rstd = l->d_rstd; p.xhat8 = l->xhat8; p.y8 = l->y8; p.y_max = l->d_y_absmax;
+    p.M = l->M; p.N = l->N; p.eps = l->eps; p.relu = l->act == DLRM_ACT_RELU;
+    const bool wide = rows_wide(p.x, p.x_ld, size) && rows_wide(p.y, p.y_ld, size);
+    if (l->dtype == DLRM_F32) norm_fwd<float>(p, wide, as_stream(stream));
+    else norm_fwd<uint16_t>(p, wide, as_stream(stream));
+    DLRM_LAUNCH_CHECK();
+    return DLRM_OK;
+}
+
+extern "C" int dlrm_layer_norm_backward_workspace_bytes(int64_t M, int32_t N, size_t *bytes) {
+    DLRM_REQUIRE(bytes != nullptr, "bytes is NULL");
+    if (int rc = norm_shape(M, N, DLRM_F32)) return rc;
+    *bytes = sizeof(float) * 2 * (size_t)norm_bwd_parts(M, N) * (size_t)N;
+    return DLRM_OK;
+}
+
+extern "C" int dlrm_layer_norm_backward(const dlrm_layer_norm_bwd *l, void *d_workspace, size_t workspace_bytes,
+                                        dlrm_stream_t stream) {
+    DLRM_REQUIRE(l != nullptr, "layer_norm_bwd descriptor is NULL");
+    if (int rc = norm_shape(l->M, l->N, l->dtype)) return rc;
+    const int size = l->dtype == DLRM_F32 ? 4 : 2;
+    const bool params = l->d_dgamma != nullptr || l->d_dbeta != nullptr;
+    NormBwd p{};
+    int64_t parts = 0;
+    hipStream_t s = as_stream(stream);
+    if (l->M > 0) {
+        DLRM_REQUIRE(l->d_dy && l->d_dx && l->d_rstd, "NULL operand");
+        DLRM_REQUIRE((l->d_x != nullptr) != (l->xhat8.d_codes != nullptr),
+                     "exactly one of the input and the checkpoint of the normalised rows must be given");
+        DLRM_REQUIRE(l->d_x == nullptr || l->d_mean != nullptr, "the input needs the rows' means");
+        DLRM_REQUIRE(l->d_relu_mask == nullptr || l->relu_mask8.d_codes == nullptr, "two ReLU masks given");
+        DLRM_REQUIRE(l->dy_ld >= l->N && l->dx_ld >= l->N && (l->d_x == nullptr || l->x_ld >= l->N) &&
+                         (l->d_relu_mask == nullptr || l->relu_mask_ld >= l->N),
+                     "leading dimension too small");
+        DLRM_REQUIRE(rows_aligned(l->d_x, size) && rows_aligned(l->d_dy, size) && rows_aligned(l->d_dx, size) &&
+                         rows_aligned(l->d_relu_mask, size),
+                     "operand is not aligned to its elements");
+        if (l->xhat8.d_codes)
+            if (int rc = act8_check(&l->xhat8, l->N, "checkpoint of the normalised rows")) return rc;
+        if (l->relu_mask8.d_codes)
+            if (int rc = act8_check(&l->relu_mask8, l->N, "checkpoint of the output")) return rc;
+        if (params) {
+            size_t need = 0;
+            if (int rc = dlrm_layer_norm_backward_workspace_bytes(l->M, l->N, &need)) return rc;
+            DLRM_REQUIRE(d_workspace != nullptr && workspace_bytes >= need, "workspace too small: %zu < %zu", workspace_bytes, need);
+            DLRM_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, "workspace must be 16-byte aligned");
+        }
+        p.x = l->d_x; p.x_ld = l->x_ld; p.xhat8 = l->xhat8; p.mean = l->d_mean; p.rstd = l->d_rstd; p.gamma = l->d_gamma;
+        p.dy = l->d_dy; p.dy_ld = l->dy_ld; p.mask = l->d_relu_mask; p.mask_ld = l->relu_mask_ld; p.mask8 = l->relu_mask8;
+        p.dx = l->d_dx; p.dx_ld = l->dx_ld; p.dx_max = l->d_dx_absmax; p.M = l->M; p.N = l->N;
+        float *ws = static_cast<float *>(d_workspace);
+        p.part_stride = l->N;
+        p.part_g = l->d_dgamma ? ws : nullptr;
+        p.part_b = l->d_dbeta ? ws + norm_bwd_parts(l->M, l->N) * l->N : nullptr;
+        const bool wide = rows_wide(p.x, p.x_ld, size) && rows_wide(p.dy, p.dy_ld, size) && rows_wide(p.mask, p.mask_ld, size) &&
+                          rows_wide(p.dx, p.dx_ld, size);
+        if (l->dtype == DLRM_F32) norm_bwd<float>(p, wide, l->d_dgamma, l->d_dbeta, &parts, s);
+        else norm_bwd<uint16_t>(p, wide, l->d_dgamma, l->d_dbeta, &parts, s);
+        DLRM_LAUNCH_CHECK();
+        if (parts == 1) return DLRM_OK;
+    }
+    if (!params) return DLRM_OK;
+    ParamSums q{};                      // (no rows: the sums over none of them are zero)
+    q.part[0] = p.part_g; q.part[1] = p.part_b; q.out[0] = l->d_dgamma; q.out[1] = l->d_dbeta;
+    q.stride = l->N; q.parts = (int)parts; q.N = l->N;
+    hipLaunchKernelGGL(param_sums_kernel, dim3((unsigned)ceil_div(l->N, 32), 2), dim3(1024), 0, s, q);
+    DLRM_LAUNCH_CHECK();
+    return DLRM_OK;
+}

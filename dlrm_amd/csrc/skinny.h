@@ -21,9 +21,9 @@ int skinny_k_backward_weight(const float *dz, int64_t dz_ld, const float *x, int
 bool gemv_ok(const void *x, int64_t x_ld, const void *w, int K);
 int gemv_forward(const float *x, int64_t x_ld, const float *w, const float *bias, float *y, int64_t y_ld, int M, int K, int relu,
                  float *y_max, hipStream_t s);
-// dx[m,k] = dz[m] w[k], zero where mask[m,k] <= 0; dx_max (or NULL): max |dx| is folded into it
+// dx[m,k] = dz[m] w[k], zero where mask[m,k] <= 0 (or mask8, the codes of an 8-bit checkpoint; either may be NULL); dx_max (or NULL): max |dx| is folded into it
 int gemv_backward_data(const float *dz, int64_t dz_ld, const float *w, float *dx, int64_t dx_ld, const float *mask,
-                       int64_t mask_ld, int M, int K, float *dx_max, hipStream_t s);
+                       int64_t mask_ld, const int8_t *mask8, int64_t mask8_ld, int M, int K, float *dx_max, hipStream_t s);
 // the last layer of a training step in one launch: y[m] = act(x[m,:] . w + b), dy[m] = d(mean loss)/dy[m] against
 // target[m] (the mean runs over mean_over samples; relu_mask: the squared error's gradient is zero where y <= 0),
 // dx[m,k] = dy[m] w[k] where x[m,k] > 0, else zero; K <= 1024.  The three results carry the bits of gemv_forward,

@@ -1,6 +1,8 @@
 // Kernels for the two layer shapes of a DLRM that are no matrix product (see skinny.h): plain float32
 // fma chains, one pass over the large operand.
 #include "skinny.h"
+
+#include "act8.h"
 #include "loss.h"
 
 #include <stdlib.h>
@@ -140,7 +142,8 @@ __global__ __launch_bounds__(kSkThreads) void gemv_fwd_kernel(const float *__res
 __global__ __launch_bounds__(kSkThreads) void gemv_bwd_data_kernel(const float *__restrict__ dz, int64_t dz_ld,
                                                                     const float *__restrict__ w, float *__restrict__ dx,
                                                                     int64_t dx_ld, const float *__restrict__ mask,
-                                                                    int64_t mask_ld, int M, int K,
+                                                                    int64_t mask_ld, const int8_t *__restrict__ mask8,
+                                                                    int64_t mask8_ld, int M, int K,
                                                                     float *__restrict__ dx_max) {
     const int kq = K >> 2;
     const int64_t total = (int64_t)M * kq;
@@ -154,6 +157,10 @@ __global__ __launch_bounds__(kSkThreads) void gemv_bwd_data_kernel(const float *
         if (mask) {
             const float4 q = *reinterpret_cast<const float4 *>(mask + m * mask_ld + k);
             r.x = q.x > 0.f ? r.x : 0.f; r.y = q.y > 0.f ? r.y : 0.f; r.z = q.z > 0.f ? r.z : 0.f; r.w = q.w > 0.f ? r.w : 0.f;
+        } else if (mask8) {
+            const unsigned q = *reinterpret_cast<const unsigned *>(mask8 + m * mask8_ld + k);
+            r.x = act8_positive(q & 0xff) ? r.x : 0.f; r.y = act8_positive((q >> 8) & 0xff) ? r.y : 0.f;
+            r.z = act8_positive((q >> 16) & 0xff) ? r.z : 0.f; r.w = act8_positive(q >> 24) ? r.w : 0.f;
         }
         *reinterpret_cast<float4 *>(dx + m * dx_ld + k) = r;
         vmax = fmaxf(fmaxf(vmax, fmaxf(fabsf(r.x), fabsf(r.y))), fmaxf(fabsf(r.z), fabsf(r.w)));
@@ -331,11 +338,11 @@ int gemv_forward(const float *x, int64_t x_ld, const float *w, const float *bias
 }
 
 int gemv_backward_data(const float *dz, int64_t dz_ld, const float *w, float *dx, int64_t dx_ld, const float *mask,
-                       int64_t mask_ld, int M, int K, float *dx_max, hipStream_t s) {
+                       int64_t mask_ld, const int8_t *mask8, int64_t mask8_ld, int M, int K, float *dx_max, hipStream_t s) {
     const int64_t blocks = ceil_div((int64_t)M * (K / 4), kSkThreads);
     const int64_t cap = dx_max ? 2048 : 8192;     // (fewer, longer workgroups when each ends with an atomic)
     hipLaunchKernelGGL(gemv_bwd_data_kernel, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(kSkThreads), 0, s, dz, dz_ld, w,
-                       dx, dx_ld, mask, mask_ld, M, K, dx_max);
+                       dx, dx_ld, mask, mask_ld, mask8, mask8_ld, M, K, dx_max);
     DLRM_LAUNCH_CHECK();
     return DLRM_OK;
 }

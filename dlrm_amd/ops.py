@@ -198,6 +198,205 @@ def embbag_backward_apply(weight, indices, offsets, batch, grad, workspace, num_
     return workspace
 
 
+# ------------------------------------------- 8-bit activation checkpoints
+
+
+def _require_here(*ts):
+    """Device tensors of the current device (the launch goes to its current stream)."""
+    here = torch.cuda.current_device() if any(t is not None and t.is_cuda for t in ts) else None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _capi.DlrmError("dlrm_amd ops need device tensors (there is no CPU fallback)")
+        if t.device.index != here:
+            raise _capi.DlrmError("a tensor lives on cuda:%d, the current device is cuda:%d" % (t.device.index, here))
+
+
+def _rows(t, what, shape=None):
+    """Leading dimension of a [rows, cols] tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError("%s must be a row-major [rows, cols] tensor%s, got shape %s and strides %s"
+                         % (what, "" if shape is None else " of shape %s" % (tuple(shape),), tuple(t.shape), t.stride()))
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _vector(t, n, what):
+    """Address of a contiguous float32 [n] tensor (0 for None)."""
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous float32 tensor of %d elements, got %s %s" % (what, n, t.dtype, tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _act_dtype(t, what):
+    if t.dtype == torch.float32:
+        return F32
+    if t.dtype == torch.bfloat16:
+        return BF16
+    raise TypeError("%s must be float32 or bfloat16, got %s" % (what, t.dtype))
+
+
+class Act8:
+    """The 8-bit checkpoint of a [rows, cols] activation: `codes` int8 [rows, >= cols rounded up to 32] and `exps` uint8
+    [rows, >= blocks], a block being 32 consecutive columns of a row; value = code * 2^(exponent - 127), code -128 a positive
+    value that rounds to zero (dlrm_act8 in include/dlrm_amd.h).  Rows of `codes` start on 16-byte boundaries.
+    Goes wherever the backward pass takes the activation it stands for: linear_backward_weight's x, linear_backward_data's and
+    layer_norm_backward's relu_mask, and (made of the normalised rows by layer_norm_forward) layer_norm_backward's x."""
+
+    __slots__ = ("codes", "exps", "cols", "desc")
+
+    def __init__(self, codes, exps, cols):
+        blocks = (cols + 31) // 32
+        if codes.dtype != torch.int8 or exps.dtype != torch.uint8:
+            raise TypeError("codes must be int8 and exponents uint8, got %s and %s" % (codes.dtype, exps.dtype))
+        ld, exps_ld = _rows(codes, "codes"), _rows(exps, "exponents")
+        if cols < 1 or codes.shape[0] != exps.shape[0] or codes.shape[1] < 32 * blocks or exps.shape[1] < blocks:
+            raise ValueError("%d columns need codes [rows, %d] and exponents [rows, %d], got %s and %s"
+                             % (cols, 32 * blocks, blocks, tuple(codes.shape), tuple(exps.shape)))
+        if codes.shape[0] == 1:
+            ld = (ld + 15) // 16 * 16
+        if ld % 16 or codes.data_ptr() % 16:
+            raise ValueError("rows of codes must start on 16-byte boundaries")
+        self.codes, self.exps, self.cols = codes, exps, cols
+        self.desc = _capi.Act8Desc(codes.data_ptr(), ld, exps.data_ptr(), exps_ld)
+
+    @staticmethod
+    def empty(rows, cols, device="cuda"):
+        blocks = (cols + 31) // 32
+        return Act8(torch.empty((rows, 32 * blocks), dtype=torch.int8, device=device),
+                    torch.empty((rows, blocks), dtype=torch.uint8, device=device), cols)
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.cols)
+
+
+def _act8(a, shape, what):
+    """Descriptor of a checkpoint that must have this shape."""
+    if not isinstance(a, Act8):
+        raise TypeError("%s must be an Act8, got %s" % (what, type(a).__name__))
+    if a.shape != tuple(shape):
+        raise ValueError("%s is a checkpoint of shape %s, expected %s" % (what, a.shape, tuple(shape)))
+    _require_here(a.codes, a.exps)
+    return a.desc
+
+
+@_op
+def act8_pack(x, out=None):
+    """The 8-bit checkpoint of a float32 or bf16 activation [rows, cols] (rows may be strided)."""
+    _require_here(x)
+    ld = _rows(x, "x")
+    if out is None:
+        out = Act8.empty(x.shape[0], x.shape[1], x.device)
+    d = _act8(out, x.shape, "out")
+    _emit("act8_pack", _ptr(x), C.c_int32(_act_dtype(x, "x")), C.c_int64(x.shape[0]), C.c_int32(x.shape[1]), C.c_int64(ld), d)
+    return out
+
+
+@_op
+def act8_unpack(a, out=None, dtype=torch.float32):
+    """The values of a checkpoint as a float32 or bf16 tensor (both hold them exactly)."""
+    if out is None:
+        out = torch.empty(a.shape, dtype=dtype, device=a.codes.device)
+    _require_here(out)
+    ld = _rows(out, "out", a.shape)
+    d = _act8(a, a.shape, "the checkpoint")
+    _emit("act8_unpack", d, C.c_int64(a.shape[0]), C.c_int32(a.cols), _ptr(out), C.c_int32(_act_dtype(out, "out")), C.c_int64(ld))
+    return out
+
+
+# ------------------------------------------------------------- layer norm
+
+
+@_op
+def layer_norm_forward(x, gamma=None, beta=None, eps=1e-5, relu=False, out=None, mean=None, rstd=None, want_stats=True,
+                       xhat8=None, y8=None, y_absmax=None):
+    """Layer norm over the rows of x [M,N] (float32 or bf16; rows may be strided): y = act(gamma xh + beta) with
+    xh = (x - mean) rstd.  Returns (y, mean, rstd); want_stats=False computes the statistics only where a buffer is given.
+    xhat8 / y8: Act8 checkpoints of xh and of y that are written in the same pass for layer_norm_backward and for the next
+    layer's backward pass.  y_absmax: see linear_forward.  out may be x."""
+    _require_here(x, gamma, beta, out, mean, rstd, y_absmax)
+    M, N = x.shape
+    d = _capi.LayerNormDesc()
+    d.M, d.N, d.dtype = M, N, _act_dtype(x, "x")
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    elif out.dtype != x.dtype:
+        raise TypeError("out must be %s like x, got %s" % (x.dtype, out.dtype))
+    if want_stats:
+        mean = torch.empty(M, dtype=torch.float32, device=x.device) if mean is None else mean
+        rstd = torch.empty(M, dtype=torch.float32, device=x.device) if rstd is None else rstd
+    d.d_x, d.x_ld = x.data_ptr(), _rows(x, "x")
+    d.d_y, d.y_ld = out.data_ptr(), _rows(out, "out", x.shape)
+    d.d_gamma, d.d_beta = _vector(gamma, N, "gamma"), _vector(beta, N, "beta")
+    d.d_mean, d.d_rstd = _vector(mean, M, "mean"), _vector(rstd, M, "rstd")
+    if xhat8 is not None:
+        d.xhat8 = _act8(xhat8, x.shape, "xhat8")
+    if y8 is not None:
+        d.y8 = _act8(y8, x.shape, "y8")
+    d.d_y_absmax = _vector(y_absmax, 1, "y_absmax")
+    d.eps, d.act = eps, _capi.ACT_RELU if relu else _capi.ACT_NONE
+    _emit("layer_norm_forward", d)
+    return out, mean, rstd
+
+
+def layer_norm_backward_workspace_bytes(M, N):
+    n = C.c_size_t(0)
+    check(_capi.lib().dlrm_layer_norm_backward_workspace_bytes(C.c_int64(M), N, C.byref(n)))
+    return int(n.value)
+
+
+@_op
+def layer_norm_backward(dy, x, rstd, mean=None, gamma=None, relu_mask=None, out=None, dgamma=None, dbeta=None,
+                        workspace=None, want_params=True, dx_absmax=None):
+    """Backward pass of layer_norm_forward.  x: its input (with mean) or the Act8 of the normalised rows; relu_mask: its output
+    or that output's Act8 where it had relu=True, else None.  Returns (dx, dgamma, dbeta, workspace); want_params=False
+    computes the parameters' gradients only where a buffer is given.  out may be dy."""
+    _require_here(dy, rstd, mean, gamma, out, dgamma, dbeta, workspace, dx_absmax)
+    M, N = dy.shape
+    d = _capi.LayerNormBwdDesc()
+    d.M, d.N, d.dtype = M, N, _act_dtype(dy, "dy")
+    if isinstance(x, Act8):
+        if mean is not None:
+            raise ValueError("the checkpoint holds normalised rows: mean has no use")
+        d.xhat8 = _act8(x, dy.shape, "x")
+    else:
+        _require_here(x)
+        if x.dtype != dy.dtype:
+            raise TypeError("x must be %s like dy, got %s" % (dy.dtype, x.dtype))
+        if mean is None:
+            raise ValueError("x needs the rows' means")
+        d.d_x, d.x_ld = x.data_ptr(), _rows(x, "x", dy.shape)
+        d.d_mean = _vector(mean, M, "mean")
+    if isinstance(relu_mask, Act8):
+        d.relu_mask8 = _act8(relu_mask, dy.shape, "relu_mask")
+    elif relu_mask is not None:
+        _require_here(relu_mask)
+        if relu_mask.dtype != dy.dtype:
+            raise TypeError("relu_mask must be %s like dy, got %s" % (dy.dtype, relu_mask.dtype))
+        d.d_relu_mask, d.relu_mask_ld = relu_mask.data_ptr(), _rows(relu_mask, "relu_mask", dy.shape)
+    if out is None:
+        out = torch.empty((M, N), dtype=dy.dtype, device=dy.device)
+    elif out.dtype != dy.dtype:
+        raise TypeError("out must be %s like dy, got %s" % (dy.dtype, out.dtype))
+    if want_params:
+        dgamma = torch.empty(N, dtype=torch.float32, device=dy.device) if dgamma is None else dgamma
+        dbeta = torch.empty(N, dtype=torch.float32, device=dy.device) if dbeta is None else dbeta
+    d.d_rstd, d.d_gamma = _vector(rstd, M, "rstd"), _vector(gamma, N, "gamma")
+    d.d_dy, d.dy_ld = dy.data_ptr(), _rows(dy, "dy")
+    d.d_dx, d.dx_ld = out.data_ptr(), _rows(out, "out", dy.shape)
+    d.d_dgamma, d.d_dbeta = _vector(dgamma, N, "dgamma"), _vector(dbeta, N, "dbeta")
+    d.d_dx_absmax = _vector(dx_absmax, 1, "dx_absmax")
+    if dgamma is not None or dbeta is not None:
+        need = layer_norm_backward_workspace_bytes(M, N)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
+    _emit("layer_norm_backward", d, _ptr(workspace), C.c_size_t(0 if workspace is None else workspace.numel()))
+    return out, dgamma, dbeta, workspace
+
+
 # ------------------------------------------------------------------ dense
 
 
@@ -261,7 +460,11 @@ def linear_forward(x, w, bias, relu, out=None, x_absmax=None, w_absmax=None, y_a
 
 @_op
 def linear_backward_data(dz, w, relu_mask=None, out=None, dz_absmax=None, w_absmax=None, dx_absmax=None, w_planes=None):
-    """dx = dz W, optionally masked with (relu_mask > 0).  *_absmax, w_planes: see linear_forward."""
+    """dx = dz W, optionally masked with (relu_mask > 0); relu_mask may be the Act8 of the activation.  *_absmax, w_planes: see
+    linear_forward."""
+    mask8 = relu_mask if isinstance(relu_mask, Act8) else None
+    if mask8 is not None:
+        relu_mask = None
     _require_cuda(dz, w, relu_mask, out)
     M, N = dz.shape
     K = w.shape[1]
@@ -274,6 +477,8 @@ def linear_backward_data(dz, w, relu_mask=None, out=None, dz_absmax=None, w_absm
     d.d_dx, d.dx_ld = out.data_ptr(), _ld(out)
     if relu_mask is not None:
         d.d_relu_mask, d.relu_mask_ld = relu_mask.data_ptr(), _ld(relu_mask)
+    elif mask8 is not None:
+        d.relu_mask8 = _act8(mask8, (M, K), "relu_mask")
     d.gemm_mode = _gemm_field()
     d.d_dz_absmax, d.d_w_absmax, d.d_dx_absmax = _ptr0(dz_absmax), _ptr0(w_absmax), _ptr0(dx_absmax)
     if w_planes is not None:
@@ -303,8 +508,9 @@ def linear_backward_weight_workspace_bytes(M, N, K):
 
 @_op
 def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True, dz_absmax=None, x_absmax=None):
-    """dW = dz^T x [N,K], db = column sums of dz.  *_absmax: see linear_forward."""
-    _require_cuda(dz, x, dw, db, workspace)
+    """dW = dz^T x [N,K], db = column sums of dz.  x may be the Act8 of the activation.  *_absmax: see linear_forward."""
+    x8 = x if isinstance(x, Act8) else None
+    _require_cuda(dz, x.codes if x8 is not None else x, dw, db, workspace)
     M, N = dz.shape
     K = x.shape[1]
     if dw is None:
@@ -317,7 +523,10 @@ def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True
     d = _capi.LinearBwdDesc()
     d.M, d.N, d.K = M, N, K
     d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
-    d.d_x, d.x_ld = x.data_ptr(), _ld(x)
+    if x8 is not None:
+        d.x8 = _act8(x8, (M, K), "x")
+    else:
+        d.d_x, d.x_ld = x.data_ptr(), _ld(x)
     d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)
     d.d_db = 0 if db is None else db.data_ptr()
     d.gemm_mode = _gemm_field()
@@ -329,13 +538,17 @@ def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True
 def linear_backward_weight_static(dz, x, dw, db=None):
     """linear_backward_weight through the entry point that allocates nothing: partial sums go to the library's
     static device array (layers beyond its size are refused); outputs must be given."""
-    _require_cuda(dz, x, dw, db)
+    x8 = x if isinstance(x, Act8) else None
+    _require_cuda(dz, x.codes if x8 is not None else x, dw, db)
     M, N = dz.shape
     K = x.shape[1]
     d = _capi.LinearBwdDesc()
     d.M, d.N, d.K = M, N, K
     d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
-    d.d_x, d.x_ld = x.data_ptr(), _ld(x)
+    if x8 is not None:
+        d.x8 = _act8(x8, (M, K), "x")
+    else:
+        d.d_x, d.x_ld = x.data_ptr(), _ld(x)
     d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)
     d.d_db = 0 if db is None else db.data_ptr()
     d.gemm_mode = _gemm_field()

@@ -19,7 +19,8 @@ from ._capi import check
 
 OP_NAMES = ("embbag_forward", "embbag_backward_update", "linear_forward", "linear_backward_data",
             "linear_backward_weight", "sgd_step", "interact_dot_forward", "interact_dot_backward", "loss", "copy_2d",
-            "embbag_backward_prepare", "embbag_backward_apply")
+            "embbag_backward_prepare", "embbag_backward_apply", "act8_pack", "act8_unpack", "layer_norm_forward",
+            "layer_norm_backward")
 
 
 class StepPlan:
@@ -92,7 +93,7 @@ class StepRecorder:
     def note(self, name, args, kwargs):
         self._call = (name, args, kwargs)
         for a in list(args) + list(kwargs.values()):
-            if isinstance(a, torch.Tensor):
+            if isinstance(a, (torch.Tensor, ops.Act8)):
                 self.plan.keep.append(a)
 
     def add(self, name, args):

@@ -7,7 +7,8 @@
  * dlrm_libtorch/include/data.h, and src/dlrmtest2.cpp with include/data2.h for the
  * second cache policy); each entry point cites the reference interface it stands in for.
  *
- * Sections: tables - EmbeddingBag (forward, fused sparse update) - MLP layers - interaction and losses -
+ * Sections: tables - EmbeddingBag (forward, fused sparse update) - 8-bit activation checkpoints - MLP layers -
+ * layer norm - interaction and losses -
  * page-LRU cache (dlrm_cache: declarations, then its calls further down) - Criteo record decode - recorded
  * step (dlrm_plan) - vector-granular cache (dlrm_vcache) - collectives (dlrm_comm) - whole model (dlrm_model).
  *
@@ -55,7 +56,7 @@ const char *dlrm_last_error(void);
  * dlrm_version() is what the loaded library was built with; a caller compiled against another
  * DLRM_ABI_VERSION must not pass structs to it (the adapter and the Python binding check this
  * before their first call). */
-#define DLRM_ABI_VERSION 1018
+#define DLRM_ABI_VERSION 1019
 int dlrm_version(void);
 /* Name of the device architecture the kernels were built for ("gfx950"). */
 const char *dlrm_target_arch(void);
@@ -175,6 +176,41 @@ int dlrm_embbag_backward_prepare(const dlrm_embbag *e, void *d_workspace, size_t
 int dlrm_embbag_backward_apply(const dlrm_embbag *e, const float *d_grad, int64_t grad_ld, const dlrm_sparse_opt *opt,
                                void *d_workspace, size_t workspace_bytes, dlrm_stream_t stream);
 
+/* ------------------------------------------- 8-bit activation checkpoints */
+
+/*
+ * An activation [rows, cols] kept for the backward pass in 8 bits (no counterpart in the reference, whose autograd
+ * keeps every activation in float32): one signed byte per element and one exponent byte per block of 32 consecutive
+ * columns of a row, 1.03 bytes an element.
+ *
+ *   block of 32 columns (the last one may be short):  E = the smallest of 1 .. 248 with max |x| < 127.5 * 2^(E-127)
+ *   code  = x / 2^(E-127), rounded to the nearest integer, ties to even: -127 .. 127
+ *   value = code * 2^(E-127): within half a step of x, i.e. within max |x| / 127.5 of the block (blocks whose values
+ *           are all below 2^-120 keep the step 2^-126; from 127.5 * 2^121 on, half a per cent below the largest float32,
+ *           the step stays 2^121 and the codes end at 127, so that every finite x keeps a finite value)
+ *   code -128: x > 0 that rounds to zero.  Its value is 0 and it still counts as positive where the checkpoint of a
+ *           ReLU's output stands in for the output as a mask, so such masks are exact.
+ *   E = 255: the block holds an infinity or a NaN; every value of it reads as NaN.
+ *
+ * Every value is an exact bf16 (and float32) number.  d_codes: 16-byte aligned, ld a multiple of 16 and at least cols
+ * rounded up to 32 (the columns behind `cols` are written as zeros and never read as values); d_exps: exps_ld at least
+ * the number of blocks.
+ */
+typedef struct dlrm_act8 {
+    int8_t *d_codes;     /* [rows, ld] */
+    int64_t ld;
+    uint8_t *d_exps;     /* [rows, exps_ld] */
+    int64_t exps_ld;
+} dlrm_act8;
+
+/* A [rows, cols] activation of dtype DLRM_F32 or DLRM_BF16 into a checkpoint, and the values of a checkpoint back into
+ * such a tensor (float32 and bf16 hold them exactly).  Rows may have any stride; rows on 16-byte boundaries are moved
+ * 16 bytes at a time.  The packing direction writes whole blocks, the unpacking one exactly cols elements a row. */
+int dlrm_act8_pack(const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld, const dlrm_act8 *out,
+                   dlrm_stream_t stream);
+int dlrm_act8_unpack(const dlrm_act8 *a, int64_t rows, int32_t cols, void *d_x, int32_t dtype, int64_t x_ld,
+                     dlrm_stream_t stream);
+
 /* ------------------------------------------------------------- dense MLP */
 
 /*
@@ -275,11 +311,18 @@ int dlrm_absmax(const float *d_x, int64_t rows, int32_t cols, int64_t ld, float 
  *                    dx = (relu_mask > 0) ? dx : 0  -- relu_mask is the output
  *                    of the previous layer (= this layer's x), which turns dx
  *                    directly into the previous layer's dz.
+ *                    relu_mask8 (d_codes != NULL) is the 8-bit checkpoint of
+ *                    that output in d_relu_mask's place, with the same result.
  *   backward_weight: dW = dz^T x  [N,K] and, if d_db != NULL, db = column
  *                    sums of dz.  The reduction over the batch is split over
  *                    workgroups; partial sums go through d_workspace
  *                    (dlrm_linear_backward_weight_workspace_bytes) and are
  *                    combined in a fixed order (reproducible).
+ *                    x8 (d_codes != NULL) is the 8-bit checkpoint of x in
+ *                    d_x's place: the product with the values it stands for.
+ *                    They are exact bf16 numbers, so dz alone is cut into its
+ *                    three bf16 pieces and the product has float32 accuracy
+ *                    from three bf16 terms; gemm_mode has no say in it.
  */
 typedef struct dlrm_linear_bwd {
     int64_t M;
@@ -304,6 +347,8 @@ typedef struct dlrm_linear_bwd {
     float *d_dx_absmax;
     /* DLRM_GEMM_F16X2 only, may be NULL: the pre-split planes of d_w (backward_data; see dlrm_linear) */
     const dlrm_weight_planes *w_planes;
+    dlrm_act8 x8;         /* [M,K] (backward_weight): instead of d_x, which must then be NULL */
+    dlrm_act8 relu_mask8; /* [M,K] (backward_data): instead of d_relu_mask, which must then be NULL */
 } dlrm_linear_bwd;
 
 int dlrm_linear_backward_data(const dlrm_linear_bwd *l, dlrm_stream_t stream);
@@ -331,6 +376,75 @@ int dlrm_linear_backward_weight_static(const dlrm_linear_bwd *l, dlrm_stream_t s
  * batch, so its momentum buffer never carries over and the step is plain SGD.
  */
 int dlrm_sgd_step(float *d_w, const float *d_g, int64_t n, float lr, dlrm_stream_t stream);
+
+/* ------------------------------------------------------------- layer norm */
+
+/*
+ * Layer norm over the rows of an activation, for MLPs that normalise between a linear layer and its ReLU (no
+ * counterpart in the reference, whose layers are Linear + ReLU alone, src/dlrmtest.cpp:254-272):
+ *
+ *   mean = sum x / N,  rstd = 1 / sqrt(sum (x - mean)^2 / N + eps),  xh = (x - mean) rstd,  y = act(gamma xh + beta)
+ *
+ * x and y are DLRM_F32 or DLRM_BF16 (`dtype`); statistics and arithmetic are float32, y is rounded once.  Any row
+ * stride is accepted, no element behind column N-1 is read or written, and d_y may be d_x itself; rows on 16-byte
+ * boundaries take 16-byte loads and stores.  DLRM_ACT_RELU passes a NaN on.
+ * What the backward pass needs can leave with the same pass: the statistics, the checkpoint of xh (xhat8) and that of
+ * the stored y (y8, equal to what dlrm_act8_pack makes of y); each is skipped where its pointer is NULL.
+ */
+typedef struct dlrm_layer_norm {
+    int64_t M;             /* rows */
+    int32_t N;             /* columns */
+    int32_t dtype;         /* of x and y: DLRM_F32 | DLRM_BF16 */
+    const void *d_x;       /* [M,N] */
+    int64_t x_ld;
+    const float *d_gamma;  /* [N] or NULL (1) */
+    const float *d_beta;   /* [N] or NULL (0) */
+    void *d_y;             /* [M,N] */
+    int64_t y_ld;
+    float *d_mean;         /* [M] or NULL */
+    float *d_rstd;         /* [M] or NULL */
+    dlrm_act8 xhat8;       /* [M,N], d_codes NULL: not written */
+    dlrm_act8 y8;          /* [M,N], d_codes NULL: not written */
+    float *d_y_absmax;     /* or NULL: max |y| is folded in with atomicMax (start it at 0; see dlrm_linear) */
+    float eps;
+    int32_t act;           /* DLRM_ACT_NONE | DLRM_ACT_RELU */
+} dlrm_layer_norm;
+
+int dlrm_layer_norm_forward(const dlrm_layer_norm *l, dlrm_stream_t stream);
+
+/*
+ * Its backward pass:  d = dy, zero where the ReLU's output was not positive (d_relu_mask = y, or relu_mask8 = its
+ * checkpoint; neither: no ReLU),
+ *   dx = rstd (gamma d - sum(gamma d) / N - xh sum(gamma d xh) / N),   dgamma = sum over rows of d xh,   dbeta = of d
+ * xh comes from d_x with d_mean, or from the checkpoint the forward pass left (xhat8; d_x and d_mean NULL).  dy, dx, x
+ * and y share `dtype`, the parameters' gradients are float32 and skipped where NULL.  d_dx may be d_dy itself.
+ * d_workspace: dlrm_layer_norm_backward_workspace_bytes() bytes of device scratch for the partial sums of the parameter
+ * gradients (NULL if neither is wanted), which are added in a fixed order (reproducible).  M = 0 gives zero gradients.
+ */
+typedef struct dlrm_layer_norm_bwd {
+    int64_t M;
+    int32_t N;
+    int32_t dtype;             /* of x, y, dy and dx */
+    const void *d_x;           /* [M,N] or NULL */
+    int64_t x_ld;
+    dlrm_act8 xhat8;           /* [M,N] in place of d_x */
+    const float *d_mean;       /* [M] (with d_x) */
+    const float *d_rstd;       /* [M] */
+    const float *d_gamma;      /* [N] or NULL (1) */
+    const void *d_dy;          /* [M,N] */
+    int64_t dy_ld;
+    const void *d_relu_mask;   /* [M,N] or NULL */
+    int64_t relu_mask_ld;
+    dlrm_act8 relu_mask8;      /* [M,N] in place of d_relu_mask */
+    void *d_dx;                /* [M,N] */
+    int64_t dx_ld;
+    float *d_dgamma;           /* [N] or NULL */
+    float *d_dbeta;            /* [N] or NULL */
+    float *d_dx_absmax;        /* or NULL: max |dx| is folded in with atomicMax */
+} dlrm_layer_norm_bwd;
+
+int dlrm_layer_norm_backward_workspace_bytes(int64_t M, int32_t N, size_t *bytes);
+int dlrm_layer_norm_backward(const dlrm_layer_norm_bwd *l, void *d_workspace, size_t workspace_bytes, dlrm_stream_t stream);
 
 /* ------------------------------------------------- interaction and losses */
 
@@ -535,7 +649,8 @@ enum {
     DLRM_OP_EMBBAG_FORWARD = 0, DLRM_OP_EMBBAG_BACKWARD_UPDATE = 1, DLRM_OP_LINEAR_FORWARD = 2,
     DLRM_OP_LINEAR_BACKWARD_DATA = 3, DLRM_OP_LINEAR_BACKWARD_WEIGHT = 4, DLRM_OP_SGD_STEP = 5,
     DLRM_OP_INTERACT_DOT_FORWARD = 6, DLRM_OP_INTERACT_DOT_BACKWARD = 7, DLRM_OP_LOSS = 8, DLRM_OP_COPY_2D = 9,
-    DLRM_OP_EMBBAG_BACKWARD_PREPARE = 10, DLRM_OP_EMBBAG_BACKWARD_APPLY = 11
+    DLRM_OP_EMBBAG_BACKWARD_PREPARE = 10, DLRM_OP_EMBBAG_BACKWARD_APPLY = 11, DLRM_OP_ACT8_PACK = 12,
+    DLRM_OP_ACT8_UNPACK = 13, DLRM_OP_LAYER_NORM_FORWARD = 14, DLRM_OP_LAYER_NORM_BACKWARD = 15
 };
 int dlrm_plan_create(dlrm_plan **out);
 int dlrm_plan_destroy(dlrm_plan *p);
@@ -567,6 +682,12 @@ int dlrm_plan_add_loss_bce_logits(dlrm_plan *p, const float *d_logit, const floa
                                   int64_t mean_over, float *d_loss, float *d_dlogit);
 int dlrm_plan_add_copy_2d(dlrm_plan *p, float *d_dst, int64_t dst_ld, const float *d_src, int64_t src_ld, int64_t rows,
                           int64_t cols);
+int dlrm_plan_add_act8_pack(dlrm_plan *p, const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld,
+                            const dlrm_act8 *out);
+int dlrm_plan_add_act8_unpack(dlrm_plan *p, const dlrm_act8 *a, int64_t rows, int32_t cols, void *d_x, int32_t dtype,
+                              int64_t x_ld);
+int dlrm_plan_add_layer_norm_forward(dlrm_plan *p, const dlrm_layer_norm *l);
+int dlrm_plan_add_layer_norm_backward(dlrm_plan *p, const dlrm_layer_norm_bwd *l, void *d_workspace, size_t workspace_bytes);
 int dlrm_plan_enable_timing(dlrm_plan *p, int32_t max_runs);
 int dlrm_plan_run(dlrm_plan *p, int32_t first, int32_t last, dlrm_stream_t stream);
 int dlrm_plan_collect_timing(dlrm_plan *p, double *h_ms_sum, int32_t *h_runs);
