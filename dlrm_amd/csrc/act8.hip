@@ -32,69 +32,81 @@ struct Act8Pass {
     int lanes_log2;        // lanes that share a row: 2^lanes_log2, a wave at most
 };
 
-template <typename T, int VEC>
+// S: steps that a lane takes per row, 4 meaning "four at a time, as often as the row needs"; with S = 1 or 2 it takes four
+// or two rows at a time, so that four loads are in flight per lane whatever the row's width
+template <typename T, int S>
 __global__ __launch_bounds__(256) void act8_pack_kernel(Act8Pass p) {
+    constexpr int VEC = kWide<T>, R = 4 / S;
     const int lane = threadIdx.x & 63, lanes = 1 << p.lanes_log2;
     const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC, width = p.blocks * kAct8Block;
     const int rows_per_wave = 64 >> p.lanes_log2;
     const int64_t n_waves = (int64_t)gridDim.x * 4;
-    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave; r0 < p.rows; r0 += n_waves * rows_per_wave) {
-        const int64_t mine = r0 + (lane >> p.lanes_log2);
-        const bool live = mine < p.rows;
-        const int64_t r = live ? mine : p.rows - 1;
-        const T *row = static_cast<const T *>(p.src) + r * p.ld;
-        int8_t *codes = p.codes + r * p.codes_ld;
-        uint8_t *exps = p.exps + r * p.exps_ld;
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave * R; r0 < p.rows; r0 += n_waves * rows_per_wave * R) {
         // (every lane of the wave takes every turn: the exchanges inside act8_store need the neighbours)
-        for (int base = 0; base < width; base += 4 * step) {
-            float v[4][VEC];
+        for (int base = 0; base < width; base += S * step) {
+            u32x4 x[4];
+            int64_t row[R];
+            bool live[R];
 #pragma unroll
-            for (int u = 0; u < 4; u++) load_elems<T, VEC>(row, base + u * step + first, p.cols, v[u]);
+            for (int k = 0; k < R; k++) {
+                row[k] = r0 + k * rows_per_wave + (lane >> p.lanes_log2);
+                live[k] = row[k] < p.rows;
+                if (!live[k]) row[k] = p.rows - 1;
+            }
 #pragma unroll
             for (int u = 0; u < 4; u++)
-                if (base + u * step < width) act8_store<VEC>(v[u], codes, exps, base + u * step + first, p.blocks, live);
+                x[u] = request_elems<T, VEC>(static_cast<const T *>(p.src) + row[u / S] * p.ld, base + (u % S) * step + first, p.cols);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int c = base + (u % S) * step + first;
+                float v[VEC];
+                elems_of<T, VEC>(x[u], c, p.cols, v);
+                act8_store<VEC>(v, p.codes + row[u / S] * p.codes_ld, p.exps + row[u / S] * p.exps_ld, c, p.blocks, live[u / S]);
+            }
         }
     }
 }
 
-template <typename T, int VEC>
+template <typename T, int S>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(Act8Pass p) {
+    constexpr int VEC = kWide<T>, R = 4 / S;
     const int lane = threadIdx.x & 63, lanes = 1 << p.lanes_log2;
     const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC;
     const int rows_per_wave = 64 >> p.lanes_log2;
     const int64_t n_waves = (int64_t)gridDim.x * 4;
-    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave; r0 < p.rows; r0 += n_waves * rows_per_wave) {
-        const int64_t r = r0 + (lane >> p.lanes_log2);
-        if (r >= p.rows) continue;
-        T *row = static_cast<T *>(p.dst) + r * p.ld;
-        const int8_t *codes = p.codes + r * p.codes_ld;
-        const uint8_t *exps = p.exps + r * p.exps_ld;
-        for (int c0 = first; c0 < p.cols; c0 += 4 * step) {
-            unsigned w[4][VEC == 8 ? 2 : 1];
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave * R; r0 < p.rows; r0 += n_waves * rows_per_wave * R) {
+        for (int base = first; base < p.cols; base += S * step) {
+            unsigned w[4][VEC / 4];
             int e[4];
+            int64_t row[R];
+#pragma unroll
+            for (int k = 0; k < R; k++) row[k] = r0 + k * rows_per_wave + (lane >> p.lanes_log2);
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int c = c0 + u * step;
-                act8_load<VEC>(codes, c, p.blocks, w[u]);
-                e[u] = c < p.cols ? exps[c / kAct8Block] : 0;
+                const int64_t r = row[u / S] < p.rows ? row[u / S] : p.rows - 1;
+                const int c = base + (u % S) * step;
+                act8_load<VEC>(p.codes + r * p.codes_ld, c, p.blocks, w[u]);
+                e[u] = p.exps[r * p.exps_ld + min(c / kAct8Block, p.blocks - 1)];
             }
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int c = c0 + u * step;
+                const int c = base + (u % S) * step;
                 float v[VEC];
                 act8_values<VEC>(w[u], act8_step(e[u]), v);
-                if (c < p.cols) store_elems<T, VEC>(row, c, p.cols, v);
+                if (c < p.cols && row[u / S] < p.rows) store_elems<T, VEC>(static_cast<T *>(p.dst) + row[u / S] * p.ld, c, p.cols, v);
             }
         }
     }
 }
 
-// lanes per row and workgroups: at least a wave's worth of steps per row is not needed, so narrow rows share a wave
-static unsigned act8_grid(Act8Pass &p, int vec) {
-    const int per_row = (int)ceil_div((int64_t)p.blocks * kAct8Block, vec);
-    p.lanes_log2 = vec == 1 ? 5 : 3;       // a block's lanes stay together
+// lanes per row (a block's stay together), steps of a lane per row and workgroups
+static unsigned act8_grid(Act8Pass &p, int vec, int *steps) {
+    const int per_row = p.blocks * (kAct8Block / vec);
+    p.lanes_log2 = vec == 8 ? 2 : 3;
     while (p.lanes_log2 < 6 && (1 << p.lanes_log2) < per_row) p.lanes_log2++;
-    const int64_t want = ceil_div(p.rows, (int64_t)4 * (64 >> p.lanes_log2));
+    const int s = (per_row + (1 << p.lanes_log2) - 1) >> p.lanes_log2;
+    *steps = s <= 2 ? s : 4;
+    const int64_t want = ceil_div(p.rows, (int64_t)4 * (64 >> p.lanes_log2) * (4 / *steps));
     return (unsigned)(want < 4096 ? want : 4096);
 }
 
@@ -119,17 +131,14 @@ static Act8Pass act8_pass(const dlrm_act8 *a, int64_t rows, int cols, int64_t x_
 
 using namespace dlrm;
 
-#define DLRM_ACT8_LAUNCH(KERNEL)                                                                                              \
-    do {                                                                                                                      \
-        const int size = dtype == DLRM_F32 ? 4 : 2;                                                                           \
-        const bool wide = reinterpret_cast<uintptr_t>(d_x) % 16 == 0 && x_ld * size % 16 == 0;                                  \
-        const unsigned grid = act8_grid(p, wide ? 16 / size : 1);                                                             \
-        hipStream_t s = as_stream(stream);                                                                                    \
-        if (dtype == DLRM_F32 && wide) hipLaunchKernelGGL((KERNEL<float, 4>), dim3(grid), dim3(256), 0, s, p);                  \
-        else if (dtype == DLRM_F32) hipLaunchKernelGGL((KERNEL<float, 1>), dim3(grid), dim3(256), 0, s, p);                     \
-        else if (wide) hipLaunchKernelGGL((KERNEL<uint16_t, 8>), dim3(grid), dim3(256), 0, s, p);                               \
-        else hipLaunchKernelGGL((KERNEL<uint16_t, 1>), dim3(grid), dim3(256), 0, s, p);                                         \
-        DLRM_LAUNCH_CHECK();                                                                                                  \
+#define DLRM_ACT8_LAUNCH(KERNEL, T)                                                                       \
+    do {                                                                                                  \
+        int steps = 1;                                                                                    \
+        const unsigned grid = act8_grid(p, kWide<T>, &steps);                                             \
+        if (steps == 1) hipLaunchKernelGGL((KERNEL<T, 1>), dim3(grid), dim3(256), 0, as_stream(stream), p);      \
+        else if (steps == 2) hipLaunchKernelGGL((KERNEL<T, 2>), dim3(grid), dim3(256), 0, as_stream(stream), p); \
+        else hipLaunchKernelGGL((KERNEL<T, 4>), dim3(grid), dim3(256), 0, as_stream(stream), p);          \
+        DLRM_LAUNCH_CHECK();                                                                              \
     } while (0)
 
 extern "C" int dlrm_act8_pack(const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld, const dlrm_act8 *out,
@@ -138,7 +147,8 @@ extern "C" int dlrm_act8_pack(const void *d_x, int32_t dtype, int64_t rows, int3
     if (rows == 0) return DLRM_OK;
     Act8Pass p = act8_pass(out, rows, cols, x_ld);
     p.src = d_x;
-    DLRM_ACT8_LAUNCH(act8_pack_kernel);
+    if (dtype == DLRM_F32) DLRM_ACT8_LAUNCH(act8_pack_kernel, float);
+    else DLRM_ACT8_LAUNCH(act8_pack_kernel, uint16_t);
     return DLRM_OK;
 }
 
@@ -148,6 +158,7 @@ extern "C" int dlrm_act8_unpack(const dlrm_act8 *a, int64_t rows, int32_t cols, 
     if (rows == 0) return DLRM_OK;
     Act8Pass p = act8_pass(a, rows, cols, x_ld);
     p.dst = d_x;
-    DLRM_ACT8_LAUNCH(act8_unpack_kernel);
+    if (dtype == DLRM_F32) DLRM_ACT8_LAUNCH(act8_unpack_kernel, float);
+    else DLRM_ACT8_LAUNCH(act8_unpack_kernel, uint16_t);
     return DLRM_OK;
 }

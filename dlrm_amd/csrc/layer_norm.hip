@@ -91,6 +91,37 @@ __device__ inline void team_sum2(float &x, float &y, float *slot) {     // slot:
     }
 }
 
+// VEC elements of gamma or beta, `none` where there is none; VEC sums to their place
+template <int VEC>
+__device__ inline void param_elems(const float *param, int c, int N, float (&v)[VEC], float none) {
+#pragma unroll
+    for (int h = 0; h < VEC; h += 4) {
+        float q[4] = {none, none, none, none};
+        if (param) elems_of<float, 4>(request_elems<float, 4>(param, c + h, N), c + h, N, q, none);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[h + j] = q[j];
+    }
+}
+template <int VEC>
+__device__ inline void store_sums(float *row, int c, int N, const float (&v)[VEC]) {
+#pragma unroll
+    for (int h = 0; h < VEC; h += 4) {
+        const float q[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+        store_elems<float, 4>(row, c + h, N, q);
+    }
+}
+
+// largest magnitude of VEC elements as they are stored
+template <typename T, int VEC>
+__device__ inline void fold_elems(const float (&v)[VEC], int c, int N, float &vmax) {
+    float t[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) t[j] = v[j];
+    round_elems<T, VEC>(t);
+#pragma unroll
+    for (int j = 0; j < VEC; j++) vmax = fmaxf(vmax, c + j < N ? fabsf(t[j]) : 0.f);
+}
+
 __device__ inline float relu_keeping_nan(float y) { return y <= 0.f ? 0.f : y; }
 
 template <typename T, int VEC>
@@ -103,38 +134,42 @@ __device__ inline void norm_output(const NormFwd &p, int64_t row, int c, bool li
     for (int j = 0; j < VEC; j++) {
         y[j] = __builtin_fmaf(xh[j], g[j], b[j]);
         if (p.relu) y[j] = relu_keeping_nan(y[j]);
-        y[j] = c + j < p.N ? rounded_to<T>(y[j]) : 0.f;
-        vmax = fmaxf(vmax, fabsf(y[j]));
     }
+    round_elems<T, VEC>(y);
+    if (c + VEC > p.N) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) y[j] = c + j < p.N ? y[j] : 0.f;
+    }
+    if (p.y_max) fold_elems<T, VEC>(y, c, p.N, vmax);
     // (the checkpoint of the stored value, so that it equals what dlrm_act8_pack makes of y)
     if (p.y8.d_codes)
         act8_store<VEC>(y, p.y8.d_codes + row * p.y8.ld, p.y8.d_exps + row * p.y8.exps_ld, c, act8_blocks(p.N), live);
     if (live) store_elems<T, VEC>(static_cast<T *>(p.y) + row * p.y_ld, c, p.N, y);
 }
 
-template <typename T, int VEC, int V, int TEAM>
+template <typename T, int V, int TEAM>
 __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(NormFwd p) {
-    constexpr int kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
+    constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
     __shared__ float slots[2][TEAM > 64 ? TEAM / 64 : 1];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     float g[V][VEC], b[V][VEC];
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int c = (v * TEAM + lane) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            g[v][j] = p.gamma && c + j < p.N ? p.gamma[c + j] : 1.f;
-            b[v][j] = p.beta && c + j < p.N ? p.beta[c + j] : 0.f;
-        }
+        param_elems<VEC>(p.gamma, c, p.N, g[v], 1.f);
+        param_elems<VEC>(p.beta, c, p.N, b[v], 0.f);
     }
     float vmax = 0.f;
     for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < p.M; r0 += (int64_t)gridDim.x * kTeams) {
         const bool live = r0 + team < p.M;            // (the other teams of the wave go along: exchanges need every lane)
         const int64_t row = live ? r0 + team : p.M - 1;
         const T *xr = static_cast<const T *>(p.x) + row * p.x_ld;
+        u32x4 raw[V];
         float x[V][VEC], s = 0.f, q = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; v++) load_elems<T, VEC>(xr, (v * TEAM + lane) * VEC, p.N, x[v]);
+        for (int v = 0; v < V; v++) raw[v] = request_elems<T, VEC>(xr, (v * TEAM + lane) * VEC, p.N);
+#pragma unroll
+        for (int v = 0; v < V; v++) elems_of<T, VEC>(raw[v], (v * TEAM + lane) * VEC, p.N, x[v]);
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
@@ -143,10 +178,17 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(Nor
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                x[v][j] = (v * TEAM + lane) * VEC + j < p.N ? x[v][j] - mean : 0.f;
-                q = __builtin_fmaf(x[v][j], x[v][j], q);
-            }
+            for (int j = 0; j < VEC; j++) x[v][j] -= mean;
+        if (p.N < V * TEAM * VEC) {        // (uniform: a row that fills its team has no columns to take out)
+#pragma unroll
+            for (int v = 0; v < V; v++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) x[v][j] = (v * TEAM + lane) * VEC + j < p.N ? x[v][j] : 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) q = __builtin_fmaf(x[v][j], x[v][j], q);
         const float rstd = 1.f / sqrtf(team_sum<TEAM>(q, slots[1]) / (float)p.N + p.eps);
         if (lane == 0 && live) {
             if (p.mean) p.mean[row] = mean;
@@ -165,8 +207,9 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(Nor
 }
 
 // rows beyond kLongRow: a workgroup of 1024 threads per row, the row read once for each sum and once for the output
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(NormFwd p) {
+    constexpr int VEC = kWide<T>;
     __shared__ float slots[2][16];
     const int first = threadIdx.x * VEC, width = act8_blocks(p.N) * kAct8Block;
     float vmax = 0.f;
@@ -175,14 +218,14 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(NormFwd p) {
         float s = 0.f, q = 0.f;
         for (int c = first; c < p.N; c += 1024 * VEC) {
             float x[VEC];
-            load_elems<T, VEC>(xr, c, p.N, x);
+            elems_of<T, VEC>(request_elems<T, VEC>(xr, c, p.N), c, p.N, x);
 #pragma unroll
             for (int j = 0; j < VEC; j++) s += x[j];
         }
         const float mean = team_sum<1024>(s, slots[0]) / (float)p.N;
         for (int c = first; c < p.N; c += 1024 * VEC) {
             float x[VEC];
-            load_elems<T, VEC>(xr, c, p.N, x);
+            elems_of<T, VEC>(request_elems<T, VEC>(xr, c, p.N), c, p.N, x);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 const float d = c + j < p.N ? x[j] - mean : 0.f;
@@ -198,63 +241,66 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(NormFwd p) {
         for (int base = 0; base < width; base += 1024 * VEC) {
             const int c = base + first;
             float x[VEC], g[VEC], b[VEC];
-            load_elems<T, VEC>(xr, c, p.N, x);
+            elems_of<T, VEC>(request_elems<T, VEC>(xr, c, p.N), c, p.N, x);
 #pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                x[j] = c + j < p.N ? (x[j] - mean) * rstd : 0.f;
-                g[j] = p.gamma && c + j < p.N ? p.gamma[c + j] : 1.f;
-                b[j] = p.beta && c + j < p.N ? p.beta[c + j] : 0.f;
-            }
+            for (int j = 0; j < VEC; j++) x[j] = c + j < p.N ? (x[j] - mean) * rstd : 0.f;
+            param_elems<VEC>(p.gamma, c, p.N, g, 1.f);
+            param_elems<VEC>(p.beta, c, p.N, b, 0.f);
             norm_output<T, VEC>(p, row, c, true, x, g, b, vmax);
         }
     }
     if (p.y_max) fold_absmax(vmax, p.y_max);
 }
 
-// xh and d of VEC elements of a row
+// What VEC elements of a row's backward pass read, requested at once, and their xh and d
 template <typename T, int VEC, bool FROM8, int MASK>
-__device__ inline void norm_grad_elems(const NormBwd &p, int64_t row, int c, float mean, float rstd, float (&xh)[VEC],
-                                       float (&d)[VEC]) {
-    const int blocks = act8_blocks(p.N);
-    if constexpr (FROM8) {
-        unsigned w[VEC == 8 ? 2 : 1];
-        act8_load<VEC>(p.xhat8.d_codes + row * p.xhat8.ld, c, blocks, w);
-        const int e = c < p.N ? p.xhat8.d_exps[row * p.xhat8.exps_ld + c / kAct8Block] : 0;
-        act8_values<VEC>(w, act8_step(e), xh);
-    } else {
-        load_elems<T, VEC>(static_cast<const T *>(p.x) + row * p.x_ld, c, p.N, xh, mean);
-#pragma unroll
-        for (int j = 0; j < VEC; j++) xh[j] = (xh[j] - mean) * rstd;
+struct NormGradPiece {
+    u32x4 x, dy, y;
+    unsigned codes[VEC / 4], marks[VEC / 4];
+    int e;
+    __device__ inline void request(const NormBwd &p, int64_t row, int c) {
+        const int blocks = act8_blocks(p.N);
+        if constexpr (FROM8) {
+            act8_load<VEC>(p.xhat8.d_codes + row * p.xhat8.ld, c, blocks, codes);
+            e = p.xhat8.d_exps[row * p.xhat8.exps_ld + min(c / kAct8Block, blocks - 1)];
+        } else x = request_elems<T, VEC>(static_cast<const T *>(p.x) + row * p.x_ld, c, p.N);
+        dy = request_elems<T, VEC>(static_cast<const T *>(p.dy) + row * p.dy_ld, c, p.N);
+        if constexpr (MASK == 1) y = request_elems<T, VEC>(static_cast<const T *>(p.mask) + row * p.mask_ld, c, p.N);
+        else if constexpr (MASK == 2) act8_load<VEC>(p.mask8.d_codes + row * p.mask8.ld, c, blocks, marks);
     }
-    load_elems<T, VEC>(static_cast<const T *>(p.dy) + row * p.dy_ld, c, p.N, d);
-    if constexpr (MASK == 1) {
-        float y[VEC];
-        load_elems<T, VEC>(static_cast<const T *>(p.mask) + row * p.mask_ld, c, p.N, y);
+    __device__ inline void values(const NormBwd &p, int c, float mean, float rstd, float (&xh)[VEC], float (&d)[VEC]) const {
+        if constexpr (FROM8) act8_values<VEC>(codes, act8_step(c < p.N ? e : 0), xh);
+        else {
+            elems_of<T, VEC>(x, c, p.N, xh, mean);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) d[j] = y[j] > 0.f ? d[j] : 0.f;
-    } else if constexpr (MASK == 2) {
-        unsigned w[VEC == 8 ? 2 : 1];
-        act8_load<VEC>(p.mask8.d_codes + row * p.mask8.ld, c, blocks, w);
+            for (int j = 0; j < VEC; j++) xh[j] = (xh[j] - mean) * rstd;
+        }
+        elems_of<T, VEC>(dy, c, p.N, d);
+        if constexpr (MASK == 1) {
+            float v[VEC];
+            elems_of<T, VEC>(y, c, p.N, v);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) d[j] = act8_positive((w[j / 4] >> (8 * (j % 4))) & 0xff) ? d[j] : 0.f;
+            for (int j = 0; j < VEC; j++) d[j] = v[j] > 0.f ? d[j] : 0.f;
+        } else if constexpr (MASK == 2) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) d[j] = act8_positive((marks[j / 4] >> (8 * (j % 4))) & 0xff) ? d[j] : 0.f;
+        }
     }
-}
+};
 
 // MASK: 0 no ReLU behind the norm, 1 its output, 2 the checkpoint of its output
-template <typename T, int VEC, int V, int TEAM, bool FROM8, int MASK>
+template <typename T, int V, int TEAM, bool FROM8, int MASK>
 __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(NormBwd p) {
-    constexpr int kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
+    constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
     __shared__ float slots[2][TEAM > 64 ? TEAM / 32 : 1];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     float g[V][VEC], acc_g[V][VEC], acc_b[V][VEC];
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int c = (v * TEAM + lane) * VEC;
+        param_elems<VEC>(p.gamma, c, p.N, g[v], 1.f);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            g[v][j] = p.gamma && c + j < p.N ? p.gamma[c + j] : 1.f;
-            acc_g[v][j] = acc_b[v][j] = 0.f;
-        }
+        for (int j = 0; j < VEC; j++) acc_g[v][j] = acc_b[v][j] = 0.f;
     }
     float vmax = 0.f;
     int turn = 0;
@@ -263,9 +309,11 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         const int64_t row = live ? r0 + team : p.M - 1;
         const float rstd = p.rstd[row], mean = FROM8 ? 0.f : p.mean[row];
         float xh[V][VEC], d[V][VEC], s1 = 0.f, s2 = 0.f;
+        NormGradPiece<T, VEC, FROM8, MASK> piece[V];
 #pragma unroll
-        for (int v = 0; v < V; v++)
-            norm_grad_elems<T, VEC, FROM8, MASK>(p, row, (v * TEAM + lane) * VEC, mean, rstd, xh[v], d[v]);
+        for (int v = 0; v < V; v++) piece[v].request(p, row, (v * TEAM + lane) * VEC);
+#pragma unroll
+        for (int v = 0; v < V; v++) piece[v].values(p, (v * TEAM + lane) * VEC, mean, rstd, xh[v], d[v]);
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
@@ -284,10 +332,8 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         for (int v = 0; v < V; v++) {
             const int c = (v * TEAM + lane) * VEC;
 #pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                d[v][j] = rounded_to<T>(rstd * (d[v][j] - c1 - xh[v][j] * c2));
-                if (c + j < p.N) vmax = fmaxf(vmax, fabsf(d[v][j]));
-            }
+            for (int j = 0; j < VEC; j++) d[v][j] = rstd * (d[v][j] - c1 - xh[v][j] * c2);
+            if (p.dx_max) fold_elems<T, VEC>(d[v], c, p.N, vmax);
             if (live) store_elems<T, VEC>(static_cast<T *>(p.dx) + row * p.dx_ld, c, p.N, d[v]);
         }
     }
@@ -316,50 +362,58 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         }
     } else {
 #pragma unroll
-        for (int v = 0; v < V; v++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                const int c = (v * TEAM + lane) * VEC + j;
-                if (c < p.N) {
-                    if (p.part_g) p.part_g[(int64_t)blockIdx.x * p.part_stride + c] = acc_g[v][j];
-                    if (p.part_b) p.part_b[(int64_t)blockIdx.x * p.part_stride + c] = acc_b[v][j];
-                }
-            }
+        for (int v = 0; v < V; v++) {
+            const int c = (v * TEAM + lane) * VEC;
+            if (p.part_g) store_sums<VEC>(p.part_g + (int64_t)blockIdx.x * p.part_stride, c, p.N, acc_g[v]);
+            if (p.part_b) store_sums<VEC>(p.part_b + (int64_t)blockIdx.x * p.part_stride, c, p.N, acc_b[v]);
+        }
     }
 }
 
-// rows beyond kLongRow.  Parameter gradients: a thread per column walks over a share of the rows (before dx is written:
+// rows beyond kLongRow.  Parameter gradients: a thread per 16 bytes of columns walks over a share of the rows (before dx is written:
 // dx may be dy's own memory) ...
 template <typename T, bool FROM8, int MASK>
 __global__ __launch_bounds__(256) void norm_bwd_long_params_kernel(NormBwd p, int64_t rows_per_part) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    constexpr int VEC = kWide<T>;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= p.N) return;
     const int64_t begin = blockIdx.y * rows_per_part;
     const int64_t end = begin + rows_per_part < p.M ? begin + rows_per_part : p.M;
-    float ag = 0.f, ab = 0.f;
+    float ag[VEC], ab[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) ag[j] = ab[j] = 0.f;
     for (int64_t row = begin; row < end; row++) {
-        float xh[1], d[1];
-        norm_grad_elems<T, 1, FROM8, MASK>(p, row, c, FROM8 ? 0.f : p.mean[row], p.rstd[row], xh, d);
-        ab += d[0];
-        ag = __builtin_fmaf(d[0], xh[0], ag);
+        float xh[VEC], d[VEC];
+        NormGradPiece<T, VEC, FROM8, MASK> piece;
+        piece.request(p, row, c);
+        piece.values(p, c, FROM8 ? 0.f : p.mean[row], p.rstd[row], xh, d);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            ab[j] += d[j];
+            ag[j] = __builtin_fmaf(d[j], xh[j], ag[j]);
+        }
     }
-    if (p.part_g) p.part_g[blockIdx.y * p.part_stride + c] = ag;
-    if (p.part_b) p.part_b[blockIdx.y * p.part_stride + c] = ab;
+    if (p.part_g) store_sums<VEC>(p.part_g + blockIdx.y * p.part_stride, c, p.N, ag);
+    if (p.part_b) store_sums<VEC>(p.part_b + blockIdx.y * p.part_stride, c, p.N, ab);
 }
 // ... and dx with a workgroup per row, which is read once for the sums and once for the output
-template <typename T, int VEC, bool FROM8, int MASK>
+template <typename T, bool FROM8, int MASK>
 __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(NormBwd p) {
+    constexpr int VEC = kWide<T>;
     __shared__ float slots[2][32];
     float vmax = 0.f;
     int turn = 0;
     for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x, turn ^= 1) {
         const float rstd = p.rstd[row], mean = FROM8 ? 0.f : p.mean[row];
-        float xh[VEC], d[VEC], s1 = 0.f, s2 = 0.f;
+        float xh[VEC], d[VEC], g[VEC], s1 = 0.f, s2 = 0.f;
         for (int c = threadIdx.x * VEC; c < p.N; c += 1024 * VEC) {
-            norm_grad_elems<T, VEC, FROM8, MASK>(p, row, c, mean, rstd, xh, d);
+            NormGradPiece<T, VEC, FROM8, MASK> piece;
+            piece.request(p, row, c);
+            piece.values(p, c, mean, rstd, xh, d);
+            param_elems<VEC>(p.gamma, c, p.N, g, 1.f);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                const float gd = p.gamma && c + j < p.N ? d[j] * p.gamma[c + j] : d[j];
+                const float gd = d[j] * g[j];
                 s1 += gd;
                 s2 = __builtin_fmaf(gd, xh[j], s2);
             }
@@ -367,13 +421,16 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(NormBwd p) {
         team_sum2<1024>(s1, s2, slots[turn]);
         const float c1 = s1 / (float)p.N, c2 = s2 / (float)p.N;
         for (int c = threadIdx.x * VEC; c < p.N; c += 1024 * VEC) {
-            norm_grad_elems<T, VEC, FROM8, MASK>(p, row, c, mean, rstd, xh, d);
+            NormGradPiece<T, VEC, FROM8, MASK> piece;
+            piece.request(p, row, c);
+            piece.values(p, c, mean, rstd, xh, d);
+            param_elems<VEC>(p.gamma, c, p.N, g, 1.f);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
-                const float gd = p.gamma && c + j < p.N ? d[j] * p.gamma[c + j] : d[j];
-                d[j] = rounded_to<T>(rstd * (gd - c1 - xh[j] * c2));
-                if (c + j < p.N) vmax = fmaxf(vmax, fabsf(d[j]));
+                const float gd = d[j] * g[j];
+                d[j] = rstd * (gd - c1 - xh[j] * c2);
             }
+            if (p.dx_max) fold_elems<T, VEC>(d, c, p.N, vmax);
             store_elems<T, VEC>(static_cast<T *>(p.dx) + row * p.dx_ld, c, p.N, d);
         }
     }
@@ -421,18 +478,18 @@ static int64_t norm_bwd_parts(int64_t M, int N) {       // most partial rows tha
     return M < cap ? (M < 1 ? 1 : M) : cap;
 }
 
-template <typename T, int VEC, int V, int TEAM>
+template <typename T, int V, int TEAM>
 static void launch_fwd(const NormFwd &p, hipStream_t s) {
     constexpr int kThreads = TEAM > 256 ? TEAM : 256;
     const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = TEAM > 256 ? 512 : 2048;
-    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((norm_fwd_kernel<T, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
 }
 
-template <typename T, int VEC, int V, int TEAM, bool FROM8, int MASK>
+template <typename T, int V, int TEAM, bool FROM8, int MASK>
 static void launch_bwd_as(const NormBwd &p, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, V, TEAM, FROM8, MASK>), dim3(grid), dim3(TEAM > 256 ? TEAM : 256), 0, s, p);
+    hipLaunchKernelGGL((norm_bwd_kernel<T, V, TEAM, FROM8, MASK>), dim3(grid), dim3(TEAM > 256 ? TEAM : 256), 0, s, p);
 }
-template <typename T, int VEC, int V, int TEAM>
+template <typename T, int V, int TEAM>
 static void launch_bwd(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
     constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM;
     const int64_t want = ceil_div(p.M, kTeams), cap = norm_bwd_parts(p.M, p.N);
@@ -444,24 +501,24 @@ static void launch_bwd(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, h
     }
     const int mask = p.mask8.d_codes ? 2 : (p.mask ? 1 : 0);
     if (p.x == nullptr) {
-        if (mask == 0) launch_bwd_as<T, VEC, V, TEAM, true, 0>(p, grid, s);
-        else if (mask == 1) launch_bwd_as<T, VEC, V, TEAM, true, 1>(p, grid, s);
-        else launch_bwd_as<T, VEC, V, TEAM, true, 2>(p, grid, s);
+        if (mask == 0) launch_bwd_as<T, V, TEAM, true, 0>(p, grid, s);
+        else if (mask == 1) launch_bwd_as<T, V, TEAM, true, 1>(p, grid, s);
+        else launch_bwd_as<T, V, TEAM, true, 2>(p, grid, s);
     } else {
-        if (mask == 0) launch_bwd_as<T, VEC, V, TEAM, false, 0>(p, grid, s);
-        else if (mask == 1) launch_bwd_as<T, VEC, V, TEAM, false, 1>(p, grid, s);
-        else launch_bwd_as<T, VEC, V, TEAM, false, 2>(p, grid, s);
+        if (mask == 0) launch_bwd_as<T, V, TEAM, false, 0>(p, grid, s);
+        else if (mask == 1) launch_bwd_as<T, V, TEAM, false, 1>(p, grid, s);
+        else launch_bwd_as<T, V, TEAM, false, 2>(p, grid, s);
     }
 }
 
-template <typename T, int VEC, bool FROM8, int MASK>
+template <typename T, bool FROM8, int MASK>
 static void launch_bwd_long_as(const NormBwd &p, int64_t parts, hipStream_t s) {
     if (p.part_g || p.part_b)
-        hipLaunchKernelGGL((norm_bwd_long_params_kernel<T, FROM8, MASK>), dim3((unsigned)ceil_div(p.N, 256), (unsigned)parts),
+        hipLaunchKernelGGL((norm_bwd_long_params_kernel<T, FROM8, MASK>), dim3((unsigned)ceil_div(p.N, 256 * kWide<T>), (unsigned)parts),
                            dim3(256), 0, s, p, ceil_div(p.M, parts));
-    hipLaunchKernelGGL((norm_bwd_long_kernel<T, VEC, FROM8, MASK>), dim3((unsigned)(p.M < 512 ? p.M : 512)), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((norm_bwd_long_kernel<T, FROM8, MASK>), dim3((unsigned)(p.M < 512 ? p.M : 512)), dim3(1024), 0, s, p);
 }
-template <typename T, int VEC>
+template <typename T>
 static void launch_bwd_long(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
     const int64_t n = ceil_div(p.M, ceil_div(p.M, norm_bwd_parts(p.M, p.N)));      // (every part has a row)
     *parts = n;
@@ -471,62 +528,47 @@ static void launch_bwd_long(NormBwd p, float *dgamma, float *dbeta, int64_t *par
     }
     const int mask = p.mask8.d_codes ? 2 : (p.mask ? 1 : 0);
     if (p.x == nullptr) {
-        if (mask == 0) launch_bwd_long_as<T, VEC, true, 0>(p, n, s);
-        else if (mask == 1) launch_bwd_long_as<T, VEC, true, 1>(p, n, s);
-        else launch_bwd_long_as<T, VEC, true, 2>(p, n, s);
+        if (mask == 0) launch_bwd_long_as<T, true, 0>(p, n, s);
+        else if (mask == 1) launch_bwd_long_as<T, true, 1>(p, n, s);
+        else launch_bwd_long_as<T, true, 2>(p, n, s);
     } else {
-        if (mask == 0) launch_bwd_long_as<T, VEC, false, 0>(p, n, s);
-        else if (mask == 1) launch_bwd_long_as<T, VEC, false, 1>(p, n, s);
-        else launch_bwd_long_as<T, VEC, false, 2>(p, n, s);
+        if (mask == 0) launch_bwd_long_as<T, false, 0>(p, n, s);
+        else if (mask == 1) launch_bwd_long_as<T, false, 1>(p, n, s);
+        else launch_bwd_long_as<T, false, 2>(p, n, s);
     }
 }
 
-// one team shape per width.  WIDE: 16 bytes a lane and step; else one element (rows that do not start on 16 bytes).
-#define DLRM_NORM_SHAPES(T, WIDE, N, CALL, LONG, ...)                          \
+// one team shape per width: the smallest that holds the row
+#define DLRM_NORM_SHAPES(T, N, CALL, LONG, ...)                                \
     do {                                                                       \
-        constexpr int W = (WIDE) ? kWide<T> : 1, F = kWide<T> / 4;             \
-        if constexpr (WIDE) {                                                  \
-            if ((N) <= 8 * W) CALL<T, W, 1, 8>(__VA_ARGS__);                   \
-            else if ((N) <= 16 * W) CALL<T, W, 1, 16>(__VA_ARGS__);            \
-            else if ((N) <= 32 * W) CALL<T, W, 1, 32>(__VA_ARGS__);            \
-            else if ((N) <= 64 * W) CALL<T, W, 1, 64>(__VA_ARGS__);            \
-            else if ((N) <= 512 * F) CALL<T, W, 2, 64>(__VA_ARGS__);           \
-            else if ((N) <= 1024 * F) CALL<T, W, 4, 64>(__VA_ARGS__);          \
-            else if ((N) <= 2048) CALL<T, W, 8 / F, 64>(__VA_ARGS__);          \
-            else if ((N) <= 4096) CALL<T, W, 4 / F, 256>(__VA_ARGS__);         \
-            else if ((N) <= 8192) CALL<T, W, 8 / F, 256>(__VA_ARGS__);         \
-            else if ((N) <= kLongRow) CALL<T, W, 4 / F, 1024>(__VA_ARGS__);    \
-            else LONG<T, W>(__VA_ARGS__);                                      \
-        } else {                                                               \
-            if ((N) <= 32) CALL<T, 1, 1, 32>(__VA_ARGS__);                     \
-            else if ((N) <= 128) CALL<T, 1, 2, 64>(__VA_ARGS__);               \
-            else if ((N) <= 512) CALL<T, 1, 8, 64>(__VA_ARGS__);               \
-            else if ((N) <= 1024) CALL<T, 1, 16, 64>(__VA_ARGS__);             \
-            else if ((N) <= 4096) CALL<T, 1, 16, 256>(__VA_ARGS__);            \
-            else if ((N) <= kLongRow) CALL<T, 1, 16, 1024>(__VA_ARGS__);       \
-            else LONG<T, 1>(__VA_ARGS__);                                      \
-        }                                                                      \
+        constexpr int W = kWide<T>, F = W / 4;                                 \
+        if ((N) <= 8 * W) CALL<T, 1, 8>(__VA_ARGS__);                          \
+        else if ((N) <= 16 * W) CALL<T, 1, 16>(__VA_ARGS__);                   \
+        else if ((N) <= 32 * W) CALL<T, 1, 32>(__VA_ARGS__);                   \
+        else if ((N) <= 64 * W) CALL<T, 1, 64>(__VA_ARGS__);                   \
+        else if ((N) <= 512 * F) CALL<T, 2, 64>(__VA_ARGS__);                  \
+        else if ((N) <= 1024 * F) CALL<T, 4, 64>(__VA_ARGS__);                 \
+        else if ((N) <= 2048) CALL<T, 8 / F, 64>(__VA_ARGS__);                 \
+        else if ((N) <= 4096) CALL<T, 4 / F, 256>(__VA_ARGS__);                \
+        else if ((N) <= 8192) CALL<T, 8 / F, 256>(__VA_ARGS__);                \
+        else if ((N) <= kLongRow) CALL<T, 4 / F, 1024>(__VA_ARGS__);           \
+        else LONG<T>(__VA_ARGS__);                                             \
     } while (0)
 
-template <typename T, int VEC>
+template <typename T>
 static void launch_fwd_long(const NormFwd &p, hipStream_t s) {
-    hipLaunchKernelGGL((norm_fwd_long_kernel<T, VEC>), dim3((unsigned)(p.M < 512 ? p.M : 512)), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((norm_fwd_long_kernel<T>), dim3((unsigned)(p.M < 512 ? p.M : 512)), dim3(1024), 0, s, p);
 }
 
 template <typename T>
-static void norm_fwd(const NormFwd &p, bool wide, hipStream_t s) {
-    if (wide) DLRM_NORM_SHAPES(T, true, p.N, launch_fwd, launch_fwd_long, p, s);
-    else DLRM_NORM_SHAPES(T, false, p.N, launch_fwd, launch_fwd_long, p, s);
+static void norm_fwd(const NormFwd &p, hipStream_t s) {
+    DLRM_NORM_SHAPES(T, p.N, launch_fwd, launch_fwd_long, p, s);
 }
 template <typename T>
-static void norm_bwd(const NormBwd &p, bool wide, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
-    if (wide) DLRM_NORM_SHAPES(T, true, p.N, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
-    else DLRM_NORM_SHAPES(T, false, p.N, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
+static void norm_bwd(const NormBwd &p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
+    DLRM_NORM_SHAPES(T, p.N, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
 }
 
-static bool rows_wide(const void *p, int64_t ld, int size) {
-    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0);
-}
 static bool rows_aligned(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
 static int norm_shape(int64_t M, int32_t N, int32_t dtype) {
@@ -557,9 +599,8 @@ extern "C" int dlrm_layer_norm_forward(const dlrm_layer_norm *l, dlrm_stream_t s
     p.x = l->d_x; p.x_ld = l->x_ld; p.gamma = l->d_gamma; p.beta = l->d_beta; p.y = l->d_y; p.y_ld = l->y_ld;
     p.mean = l->d_mean; p.rstd = l->d_rstd; p.xhat8 = l->xhat8; p.y8 = l->y8; p.y_max = l->d_y_absmax;
     p.M = l->M; p.N = l->N; p.eps = l->eps; p.relu = l->act == DLRM_ACT_RELU;
-    const bool wide = rows_wide(p.x, p.x_ld, size) && rows_wide(p.y, p.y_ld, size);
-    if (l->dtype == DLRM_F32) norm_fwd<float>(p, wide, as_stream(stream));
-    else norm_fwd<uint16_t>(p, wide, as_stream(stream));
+    if (l->dtype == DLRM_F32) norm_fwd<float>(p, as_stream(stream));
+    else norm_fwd<uint16_t>(p, as_stream(stream));
     DLRM_LAUNCH_CHECK();
     return DLRM_OK;
 }
@@ -609,10 +650,8 @@ extern "C" int dlrm_layer_norm_backward(const dlrm_layer_norm_bwd *l, void *d_wo
         p.part_stride = l->N;
         p.part_g = l->d_dgamma ? ws : nullptr;
         p.part_b = l->d_dbeta ? ws + norm_bwd_parts(l->M, l->N) * l->N : nullptr;
-        const bool wide = rows_wide(p.x, p.x_ld, size) && rows_wide(p.dy, p.dy_ld, size) && rows_wide(p.mask, p.mask_ld, size) &&
-                          rows_wide(p.dx, p.dx_ld, size);
-        if (l->dtype == DLRM_F32) norm_bwd<float>(p, wide, l->d_dgamma, l->d_dbeta, &parts, s);
-        else norm_bwd<uint16_t>(p, wide, l->d_dgamma, l->d_dbeta, &parts, s);
+        if (l->dtype == DLRM_F32) norm_bwd<float>(p, l->d_dgamma, l->d_dbeta, &parts, s);
+        else norm_bwd<uint16_t>(p, l->d_dgamma, l->d_dbeta, &parts, s);
         DLRM_LAUNCH_CHECK();
         if (parts == 1) return DLRM_OK;
     }

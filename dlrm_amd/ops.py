@@ -4,6 +4,7 @@ torch supplies device memory and the current stream only; every computation
 here is a hand-written HIP kernel inside libdlrm_amd.so.
 """
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -13,7 +14,8 @@ from ._capi import (BF16, F32, I32, I64, EmbBagDesc, SparseOpt, check)  # noqa: 
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the raw handle: building the Stream object around it costs more than the rest of a small launch's Python)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 # While a StepRecorder is installed (dlrm_amd.plan), the operators below do everything except launch:
@@ -34,8 +36,6 @@ def _emit(name, *args):
 def _op(fn):
     """Marks a public operator: a recorder learns which operator (and with which arguments) the
     entries recorded next belong to."""
-    import functools
-
     @functools.wraps(fn)
     def wrapped(*a, **kw):
         if _recorder is not None:
@@ -203,37 +203,40 @@ def embbag_backward_apply(weight, indices, offsets, batch, grad, workspace, num_
 
 def _require_here(*ts):
     """Device tensors of the current device (the launch goes to its current stream)."""
-    here = torch.cuda.current_device() if any(t is not None and t.is_cuda for t in ts) else None
+    here = None
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _capi.DlrmError("dlrm_amd ops need device tensors (there is no CPU fallback)")
-        if t.device.index != here:
-            raise _capi.DlrmError("a tensor lives on cuda:%d, the current device is cuda:%d" % (t.device.index, here))
+        if t is not None:
+            at = t.get_device()
+            if at != here:
+                if at < 0:
+                    raise _capi.DlrmError("dlrm_amd ops need device tensors (there is no CPU fallback)")
+                here = torch.cuda.current_device()
+                if at != here:
+                    raise _capi.DlrmError("a tensor lives on cuda:%d, the current device is cuda:%d" % (at, here))
 
 
 def _rows(t, what, shape=None):
     """Leading dimension of a [rows, cols] tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (shape is not None and tuple(t.shape) != tuple(shape)):
+    s, st = t.shape, t.stride()
+    if len(s) != 2 or (st[1] != 1 and s[1] > 1) or (shape is not None and s != shape):
         raise ValueError("%s must be a row-major [rows, cols] tensor%s, got shape %s and strides %s"
-                         % (what, "" if shape is None else " of shape %s" % (tuple(shape),), tuple(t.shape), t.stride()))
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+                         % (what, "" if shape is None else " of shape %s" % (tuple(shape),), tuple(s), st))
+    return st[0] if s[0] > 1 else max(st[0], s[1])
 
 
 def _vector(t, n, what):
     """Address of a contiguous float32 [n] tensor (0 for None)."""
     if t is None:
         return 0
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError("%s must be a contiguous float32 tensor of %d elements, got %s %s" % (what, n, t.dtype, tuple(t.shape)))
     return t.data_ptr()
 
 
 def _act_dtype(t, what):
-    if t.dtype == torch.float32:
+    if t.dtype is torch.float32:
         return F32
-    if t.dtype == torch.bfloat16:
+    if t.dtype is torch.bfloat16:
         return BF16
     raise TypeError("%s must be float32 or bfloat16, got %s" % (what, t.dtype))
 
@@ -245,22 +248,26 @@ class Act8:
     Goes wherever the backward pass takes the activation it stands for: linear_backward_weight's x, linear_backward_data's and
     layer_norm_backward's relu_mask, and (made of the normalised rows by layer_norm_forward) layer_norm_backward's x."""
 
-    __slots__ = ("codes", "exps", "cols", "desc")
+    __slots__ = ("codes", "exps", "cols", "shape", "desc")
 
     def __init__(self, codes, exps, cols):
-        blocks = (cols + 31) // 32
-        if codes.dtype != torch.int8 or exps.dtype != torch.uint8:
+        if codes.dtype is not torch.int8 or exps.dtype is not torch.uint8:
             raise TypeError("codes must be int8 and exponents uint8, got %s and %s" % (codes.dtype, exps.dtype))
+        blocks = (cols + 31) // 32
         ld, exps_ld = _rows(codes, "codes"), _rows(exps, "exponents")
-        if cols < 1 or codes.shape[0] != exps.shape[0] or codes.shape[1] < 32 * blocks or exps.shape[1] < blocks:
+        rows, width = codes.shape
+        if cols < 1 or exps.shape[0] != rows or width < 32 * blocks or exps.shape[1] < blocks:
             raise ValueError("%d columns need codes [rows, %d] and exponents [rows, %d], got %s and %s"
                              % (cols, 32 * blocks, blocks, tuple(codes.shape), tuple(exps.shape)))
-        if codes.shape[0] == 1:
+        if codes.get_device() != exps.get_device():
+            raise ValueError("codes and exponents live on different devices")
+        if rows == 1:
             ld = (ld + 15) // 16 * 16
-        if ld % 16 or codes.data_ptr() % 16:
+        at = codes.data_ptr()
+        if ld % 16 or at % 16:
             raise ValueError("rows of codes must start on 16-byte boundaries")
-        self.codes, self.exps, self.cols = codes, exps, cols
-        self.desc = _capi.Act8Desc(codes.data_ptr(), ld, exps.data_ptr(), exps_ld)
+        self.codes, self.exps, self.cols, self.shape = codes, exps, cols, torch.Size((rows, cols))
+        self.desc = _capi.Act8Desc(at, ld, exps.data_ptr(), exps_ld)
 
     @staticmethod
     def empty(rows, cols, device="cuda"):
@@ -268,26 +275,30 @@ class Act8:
         return Act8(torch.empty((rows, 32 * blocks), dtype=torch.int8, device=device),
                     torch.empty((rows, blocks), dtype=torch.uint8, device=device), cols)
 
-    @property
-    def shape(self):
-        return (self.codes.shape[0], self.cols)
+
+_no_act8 = _capi.Act8Desc()
 
 
 def _act8(a, shape, what):
-    """Descriptor of a checkpoint that must have this shape."""
+    """Descriptor of a checkpoint that must have this shape (None: an empty one).  The caller has checked its device."""
+    if a is None:
+        return _no_act8
     if not isinstance(a, Act8):
         raise TypeError("%s must be an Act8, got %s" % (what, type(a).__name__))
-    if a.shape != tuple(shape):
-        raise ValueError("%s is a checkpoint of shape %s, expected %s" % (what, a.shape, tuple(shape)))
-    _require_here(a.codes, a.exps)
+    if a.shape != shape:
+        raise ValueError("%s is a checkpoint of shape %s, expected %s" % (what, tuple(a.shape), tuple(shape)))
     return a.desc
+
+
+def _codes(a):
+    return a.codes if isinstance(a, Act8) else a
 
 
 @_op
 def act8_pack(x, out=None):
     """The 8-bit checkpoint of a float32 or bf16 activation [rows, cols] (rows may be strided)."""
-    _require_here(x)
     ld = _rows(x, "x")
+    _require_here(x, None if out is None else out.codes)
     if out is None:
         out = Act8.empty(x.shape[0], x.shape[1], x.device)
     d = _act8(out, x.shape, "out")
@@ -300,10 +311,10 @@ def act8_unpack(a, out=None, dtype=torch.float32):
     """The values of a checkpoint as a float32 or bf16 tensor (both hold them exactly)."""
     if out is None:
         out = torch.empty(a.shape, dtype=dtype, device=a.codes.device)
-    _require_here(out)
+    _require_here(out, a.codes)
     ld = _rows(out, "out", a.shape)
-    d = _act8(a, a.shape, "the checkpoint")
-    _emit("act8_unpack", d, C.c_int64(a.shape[0]), C.c_int32(a.cols), _ptr(out), C.c_int32(_act_dtype(out, "out")), C.c_int64(ld))
+    _emit("act8_unpack", a.desc, C.c_int64(a.shape[0]), C.c_int32(a.cols), _ptr(out), C.c_int32(_act_dtype(out, "out")),
+          C.c_int64(ld))
     return out
 
 
@@ -317,31 +328,25 @@ def layer_norm_forward(x, gamma=None, beta=None, eps=1e-5, relu=False, out=None,
     xh = (x - mean) rstd.  Returns (y, mean, rstd); want_stats=False computes the statistics only where a buffer is given.
     xhat8 / y8: Act8 checkpoints of xh and of y that are written in the same pass for layer_norm_backward and for the next
     layer's backward pass.  y_absmax: see linear_forward.  out may be x."""
-    _require_here(x, gamma, beta, out, mean, rstd, y_absmax)
-    M, N = x.shape
-    d = _capi.LayerNormDesc()
-    d.M, d.N, d.dtype = M, N, _act_dtype(x, "x")
+    _require_here(x, gamma, beta, out, mean, rstd, y_absmax, _codes(xhat8), _codes(y8))
+    x_ld = _rows(x, "x")
+    M, N = shape = x.shape
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    elif out.dtype != x.dtype:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.dtype is not x.dtype:
         raise TypeError("out must be %s like x, got %s" % (x.dtype, out.dtype))
     if want_stats:
         mean = torch.empty(M, dtype=torch.float32, device=x.device) if mean is None else mean
         rstd = torch.empty(M, dtype=torch.float32, device=x.device) if rstd is None else rstd
-    d.d_x, d.x_ld = x.data_ptr(), _rows(x, "x")
-    d.d_y, d.y_ld = out.data_ptr(), _rows(out, "out", x.shape)
-    d.d_gamma, d.d_beta = _vector(gamma, N, "gamma"), _vector(beta, N, "beta")
-    d.d_mean, d.d_rstd = _vector(mean, M, "mean"), _vector(rstd, M, "rstd")
-    if xhat8 is not None:
-        d.xhat8 = _act8(xhat8, x.shape, "xhat8")
-    if y8 is not None:
-        d.y8 = _act8(y8, x.shape, "y8")
-    d.d_y_absmax = _vector(y_absmax, 1, "y_absmax")
-    d.eps, d.act = eps, _capi.ACT_RELU if relu else _capi.ACT_NONE
-    _emit("layer_norm_forward", d)
+    _emit("layer_norm_forward", _capi.LayerNormDesc(
+        M, N, _act_dtype(x, "x"), x.data_ptr(), x_ld, _vector(gamma, N, "gamma"), _vector(beta, N, "beta"),
+        out.data_ptr(), _rows(out, "out", shape), _vector(mean, M, "mean"), _vector(rstd, M, "rstd"),
+        _act8(xhat8, shape, "xhat8"), _act8(y8, shape, "y8"), _vector(y_absmax, 1, "y_absmax"), eps,
+        _capi.ACT_RELU if relu else _capi.ACT_NONE))
     return out, mean, rstd
 
 
+@functools.lru_cache(maxsize=4096)
 def layer_norm_backward_workspace_bytes(M, N):
     n = C.c_size_t(0)
     check(_capi.lib().dlrm_layer_norm_backward_workspace_bytes(C.c_int64(M), N, C.byref(n)))
@@ -354,46 +359,45 @@ def layer_norm_backward(dy, x, rstd, mean=None, gamma=None, relu_mask=None, out=
     """Backward pass of layer_norm_forward.  x: its input (with mean) or the Act8 of the normalised rows; relu_mask: its output
     or that output's Act8 where it had relu=True, else None.  Returns (dx, dgamma, dbeta, workspace); want_params=False
     computes the parameters' gradients only where a buffer is given.  out may be dy."""
-    _require_here(dy, rstd, mean, gamma, out, dgamma, dbeta, workspace, dx_absmax)
-    M, N = dy.shape
-    d = _capi.LayerNormBwdDesc()
-    d.M, d.N, d.dtype = M, N, _act_dtype(dy, "dy")
+    _require_here(dy, rstd, mean, gamma, out, dgamma, dbeta, workspace, dx_absmax, _codes(x), _codes(relu_mask))
+    dy_ld = _rows(dy, "dy")
+    M, N = shape = dy.shape
+    dtype = _act_dtype(dy, "dy")
+    x_at = x_ld = mask_at = mask_ld = 0
+    x8 = mask8 = None
     if isinstance(x, Act8):
         if mean is not None:
             raise ValueError("the checkpoint holds normalised rows: mean has no use")
-        d.xhat8 = _act8(x, dy.shape, "x")
+        x8 = x
     else:
-        _require_here(x)
-        if x.dtype != dy.dtype:
+        if x.dtype is not dy.dtype:
             raise TypeError("x must be %s like dy, got %s" % (dy.dtype, x.dtype))
         if mean is None:
             raise ValueError("x needs the rows' means")
-        d.d_x, d.x_ld = x.data_ptr(), _rows(x, "x", dy.shape)
-        d.d_mean = _vector(mean, M, "mean")
+        x_at, x_ld = x.data_ptr(), _rows(x, "x", shape)
     if isinstance(relu_mask, Act8):
-        d.relu_mask8 = _act8(relu_mask, dy.shape, "relu_mask")
+        mask8 = relu_mask
     elif relu_mask is not None:
-        _require_here(relu_mask)
-        if relu_mask.dtype != dy.dtype:
+        if relu_mask.dtype is not dy.dtype:
             raise TypeError("relu_mask must be %s like dy, got %s" % (dy.dtype, relu_mask.dtype))
-        d.d_relu_mask, d.relu_mask_ld = relu_mask.data_ptr(), _rows(relu_mask, "relu_mask", dy.shape)
+        mask_at, mask_ld = relu_mask.data_ptr(), _rows(relu_mask, "relu_mask", shape)
     if out is None:
-        out = torch.empty((M, N), dtype=dy.dtype, device=dy.device)
-    elif out.dtype != dy.dtype:
+        out = torch.empty(shape, dtype=dy.dtype, device=dy.device)
+    elif out.dtype is not dy.dtype:
         raise TypeError("out must be %s like dy, got %s" % (dy.dtype, out.dtype))
     if want_params:
         dgamma = torch.empty(N, dtype=torch.float32, device=dy.device) if dgamma is None else dgamma
         dbeta = torch.empty(N, dtype=torch.float32, device=dy.device) if dbeta is None else dbeta
-    d.d_rstd, d.d_gamma = _vector(rstd, M, "rstd"), _vector(gamma, N, "gamma")
-    d.d_dy, d.dy_ld = dy.data_ptr(), _rows(dy, "dy")
-    d.d_dx, d.dx_ld = out.data_ptr(), _rows(out, "out", dy.shape)
-    d.d_dgamma, d.d_dbeta = _vector(dgamma, N, "dgamma"), _vector(dbeta, N, "dbeta")
-    d.d_dx_absmax = _vector(dx_absmax, 1, "dx_absmax")
     if dgamma is not None or dbeta is not None:
         need = layer_norm_backward_workspace_bytes(M, N)
         if workspace is None or workspace.numel() < need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
-    _emit("layer_norm_backward", d, _ptr(workspace), C.c_size_t(0 if workspace is None else workspace.numel()))
+    _emit("layer_norm_backward", _capi.LayerNormBwdDesc(
+        M, N, dtype, x_at, x_ld, _act8(x8, shape, "x"), _vector(mean, M, "mean"), _vector(rstd, M, "rstd"),
+        _vector(gamma, N, "gamma"), dy.data_ptr(), dy_ld, mask_at, mask_ld, _act8(mask8, shape, "relu_mask"),
+        out.data_ptr(), _rows(out, "out", shape), _vector(dgamma, N, "dgamma"), _vector(dbeta, N, "dbeta"),
+        _vector(dx_absmax, 1, "dx_absmax")),
+        _ptr(workspace), C.c_size_t(0 if workspace is None else workspace.numel()))
     return out, dgamma, dbeta, workspace
 
 
@@ -465,6 +469,7 @@ def linear_backward_data(dz, w, relu_mask=None, out=None, dz_absmax=None, w_absm
     mask8 = relu_mask if isinstance(relu_mask, Act8) else None
     if mask8 is not None:
         relu_mask = None
+        _require_here(dz, mask8.codes)
     _require_cuda(dz, w, relu_mask, out)
     M, N = dz.shape
     K = w.shape[1]
@@ -500,6 +505,7 @@ def absmax_(x, slot):
     return slot
 
 
+@functools.lru_cache(maxsize=4096)
 def linear_backward_weight_workspace_bytes(M, N, K):
     n = C.c_size_t(0)
     check(_capi.lib().dlrm_linear_backward_weight_workspace_bytes(C.c_int64(M), N, K, C.byref(n)))
@@ -510,7 +516,9 @@ def linear_backward_weight_workspace_bytes(M, N, K):
 def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True, dz_absmax=None, x_absmax=None):
     """dW = dz^T x [N,K], db = column sums of dz.  x may be the Act8 of the activation.  *_absmax: see linear_forward."""
     x8 = x if isinstance(x, Act8) else None
-    _require_cuda(dz, x.codes if x8 is not None else x, dw, db, workspace)
+    if x8 is not None:
+        _require_here(dz, x8.codes)
+    _require_cuda(dz, _codes(x), dw, db, workspace)
     M, N = dz.shape
     K = x.shape[1]
     if dw is None:
@@ -539,7 +547,9 @@ def linear_backward_weight_static(dz, x, dw, db=None):
     """linear_backward_weight through the entry point that allocates nothing: partial sums go to the library's
     static device array (layers beyond its size are refused); outputs must be given."""
     x8 = x if isinstance(x, Act8) else None
-    _require_cuda(dz, x.codes if x8 is not None else x, dw, db)
+    if x8 is not None:
+        _require_here(dz, x8.codes)
+    _require_cuda(dz, _codes(x), dw, db)
     M, N = dz.shape
     K = x.shape[1]
     d = _capi.LinearBwdDesc()
