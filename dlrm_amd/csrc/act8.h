@@ -40,7 +40,13 @@ struct Wgrad8 {
     int rows_per_split;      // a multiple of 32
     int gx, gy, gz;          // gz: ranges; gx, gy are filled in by the launch
 };
-int launch_wgrad8(Wgrad8 p, int tm, int tn, hipStream_t s);      // output tile tm x tn, each 128 or 64
+int launch_wgrad8(Wgrad8 p, int tm, int tn, hipStream_t s);
+// output tile, ranges of the batch and the bytes of their partial sums; max_bytes != 0: at most so many
+struct Wgrad8Shape {
+    int tm, tn, splits, rows_per_split;
+    size_t bytes;
+};
+Wgrad8Shape wgrad8_shape(int64_t M, int N, int K, size_t max_bytes);
 
 // exponent byte of a block whose largest magnitude has the bits `amax` (sign cleared): the mantissa carries into the
 // exponent from 127.5/128 of the next power of two on.  At most 248: 64 steps of 2^122 would be an infinity, so blocks that

@@ -5,12 +5,16 @@
 // take, every product exact in float32, float32 accumulation -- the accuracy of the bf16x3 evaluation at half its matrix
 // work and with a quarter of x's bytes.
 //
-// A 256-thread workgroup owns TM columns of dz x TN columns of x (TM, TN in {128, 64}; 2 x 2 waves, each with
-// (TM/64) x (TN/64) MFMA tiles) for a range of rows and walks it in steps of 32 rows: the next step's operands are
-// requested into registers, the present step's MFMAs run out of one LDS stage, then the requested operands are split /
-// widened to bf16 and written to the other stage.  Both operands have the reduction index as their row, so LDS holds
-// [32 rows][TM or TN] bf16 planes and the fragments come out of the transposing read ds_read_b64_tr_b16.  Row ranges
-// leave partial sums that the caller adds in a fixed order.
+// A 256-thread workgroup owns TM columns of dz x TN columns of x (2 x 2 waves, each with (TM/64) x (TN/64) MFMA tiles) for a
+// range of rows and walks it in steps of 16: the operands of the step after next are requested into registers, those of the
+// next step are cut into pieces / widened to bf16 and written to one LDS stage, the present step's MFMAs run out of the
+// other.  Both operands have the reduction index as their row, so LDS holds [16 rows][TM or TN] bf16 planes and the
+// fragments come out of the transposing read ds_read_b64_tr_b16.  Row ranges leave partial sums that the caller adds in a
+// fixed order.  x costs a third of dz's LDS traffic and half its conversions per column, so the tile is wider in x.
+//
+// What bounds it: 65536 x 1024 x 1024, 412 GF of bf16 MFMA: 339 us with the addition of the ranges (65536-row N(0,1) data),
+// 1.22 PF/s, where a large bf16 product of the library sustains 1.17 to 1.34 on the same card.  Counters at 380 us: the MFMA
+// pipe busy 55 % of the cycles at 1.87 GHz, 4.7 vector instructions per MFMA (the conversions), LDS 28 %.
 #include "act8.h"
 
 namespace dlrm {
@@ -22,9 +26,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kStepRows = 32;
+constexpr int kStepRows = 16;
 
-// byte offset of 16-byte chunk ch of row `row` in a [32][R] bf16 plane.  The transposing read takes four rows x 64 bytes
+// byte offset of 16-byte chunk ch of row `row` in a [16][R] bf16 plane.  The transposing read takes four rows x 64 bytes
 // per 32 lanes; the exchange of chunks puts those on different banks.
 template <int R>
 __device__ inline int plane_off(int row, int ch) {
@@ -32,19 +36,35 @@ __device__ inline int plane_off(int row, int ch) {
     else return 2 * R * row + 16 * (ch ^ (((row & 3) << 2) | ((row >> 2) & 3)));
 }
 
-// reduction rows 16 slice + 8 (lane / 32) .. +7 of column base + lane % 32
+// reduction rows 8 (lane / 32) .. +7 of column base + lane % 32
 template <int R>
-__device__ inline bf16x8 plane_frag(const unsigned char *plane, int base, int slice) {
+__device__ inline bf16x8 plane_frag(const unsigned char *plane, int base) {
     const int lane = threadIdx.x & 63;
     const int li = lane & 15, g = lane >> 4;
     const int ch = (base >> 3) + 2 * (g & 1) + ((li & 3) >> 1);
-    const int row = 16 * slice + 8 * (g >> 1) + (li >> 2);
+    const int row = 8 * (g >> 1) + (li >> 2);
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(plane + plane_off<R>(row, ch) + 8 * (li & 1)));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(plane + plane_off<R>(row + 4, ch) + 8 * (li & 1)));
     const s16x8 t = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(bf16x8, t);
 }
+
+// Scheduling recipe of a step: the fragment reads, then the next step's conversions spread evenly behind the MFMAs, its LDS
+// writes behind the last ones
+template <int I, int MFMAS, int VALU, int WRITES>
+__device__ inline void interleave() {
+    if constexpr (I < MFMAS) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (VALU * (I + 1)) / MFMAS - (VALU * I) / MFMAS, 0);
+        if constexpr (I == MFMAS / 2 - 1 || I == MFMAS - 1) __builtin_amdgcn_sched_group_barrier(0x200, (WRITES + 1) / 2, 0);
+        interleave<I + 1, MFMAS, VALU, WRITES>();
+    }
+}
+
+// a compiler fence for register values: their uses stay in the step they are written in
+__device__ inline void pin(f32x4 &a) { asm volatile("" : "+v"(a)); }
+__device__ inline void pin(unsigned &a) { asm volatile("" : "+v"(a)); }
 
 // two values that bf16 holds exactly, packed
 __device__ inline unsigned exact_bf16_pair(float a, float b) {
@@ -54,10 +74,9 @@ __device__ inline unsigned exact_bf16_pair(float a, float b) {
 template <int TM, int TN>
 __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     constexpr int MI = TM / 64, NI = TN / 64;
-    constexpr int PA = TM / 32, LA = TM / 4;              // dz: 16-byte pieces per thread and step, lanes per row
-    constexpr int CP = TN == 64 ? 8 : 16, LB = TN / CP;   // x: codes per piece (one per thread), lanes per row
+    constexpr int PA = TM / 64, LA = TM / 4, RA = 256 / LA;     // dz: 16-byte pieces per thread and step, lanes per row, rows per piece
+    constexpr int CP = TN / 16, LB = 16;                        // x: codes per thread and step, lanes per row
     constexpr int kPlaneA = kStepRows * TM * 2, kPlaneB = kStepRows * TN * 2, kStage = 3 * kPlaneA + kPlaneB;
-    static_assert(kStepRows * TN == 256 * CP, "one piece of x per thread and step");
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * kStage];
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -69,7 +88,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     const int bx = tile % p.gx, by = (tile / p.gx) % p.gy, bz = tile / (p.gx * p.gy);
     const int n0 = by * TM, k0 = bx * TN;
     const int begin = bz * p.rows_per_split, end = min(p.M, begin + p.rows_per_split);
-    const int steps = (end - begin + kStepRows - 1) / kStepRows;
+    const int full = (end - begin) / kStepRows, steps = (end - begin + kStepRows - 1) / kStepRows;
 
     // columns past the operands only feed outputs that are never stored: their loads are moved inside the row
     int ca = n0 + 4 * (tid % LA);
@@ -89,93 +108,142 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     const bool sums = p.colsum != nullptr && bx == 0;
     f32x4 colsum = {0.f, 0.f, 0.f, 0.f};
 
-    f32x4 xa[PA];
-    unsigned xb[CP / 4];
-    int eb;
-    auto load = [&](int t) {
+    struct Raw {                              // one step's operands on their way
+        f32x4 a[PA];
+        unsigned b[CP / 4], e;
+    };
+    // a wave-uniform origin and 32-bit offsets that no step changes (the launch bounds the row lengths)
+    const unsigned oa = ((unsigned)ra * (unsigned)p.dz_ld + (unsigned)ca) * 4u, ob = (unsigned)rb * (unsigned)p.codes_ld + (unsigned)cb;
+    const unsigned oe = (unsigned)rb * (unsigned)p.exps_ld + (unsigned)(cb / kAct8Block);
+    auto request = [&](int t, Raw &x) {       // a whole step on 16-byte boundaries
+        const int64_t r0 = begin + t * kStepRows;
+        const char *a = reinterpret_cast<const char *>(p.dz + r0 * p.dz_ld);
+        const int8_t *b = p.codes + r0 * p.codes_ld;
+#pragma unroll
+        for (int v = 0; v < PA; v++) x.a[v] = *reinterpret_cast<const f32x4 *>(a + (oa + (unsigned)(RA * v) * (unsigned)p.dz_ld * 4u));
+        if constexpr (CP == 16) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(b + ob);
+#pragma unroll
+            for (int q = 0; q < 4; q++) x.b[q] = w[q];
+        } else if constexpr (CP == 8) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(b + ob);
+            x.b[0] = w[0];
+            x.b[1] = w[1];
+        } else x.b[0] = *reinterpret_cast<const unsigned *>(b + ob);
+        x.e = (p.exps + r0 * p.exps_ld)[oe];
+    };
+    auto request_any = [&](int t, Raw &x) {   // any step: rows past the range count as zeros
         const int r0 = begin + t * kStepRows;
 #pragma unroll
         for (int v = 0; v < PA; v++) {
-            const int r = r0 + ra + (1024 / TM) * v;
+            const int r = r0 + ra + RA * v;
             const float *row = p.dz + (int64_t)min(r, end - 1) * p.dz_ld;
-            f32x4 x;
-            if (p.dz_vec) x = *reinterpret_cast<const f32x4 *>(row + ca);
-            else
 #pragma unroll
-                for (int q = 0; q < 4; q++) x[q] = row[min(ca + q, p.N - 1)];
-#pragma unroll
-            for (int q = 0; q < 4; q++) xa[v][q] = r < end ? x[q] : 0.f;
+            for (int q = 0; q < 4; q++) {
+                const float f = row[p.dz_vec ? ca + q : min(ca + q, p.N - 1)];
+                x.a[v][q] = r < end ? f : 0.f;
+            }
         }
         const int r = r0 + rb;
         const int64_t rc = min(r, end - 1);
-        if constexpr (CP == 16) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(p.codes + rc * p.codes_ld + cb);
 #pragma unroll
-            for (int q = 0; q < 4; q++) xb[q] = w[q];
-        } else {
-            const u32x2 w = *reinterpret_cast<const u32x2 *>(p.codes + rc * p.codes_ld + cb);
-            xb[0] = w[0];
-            xb[1] = w[1];
-        }
-        eb = p.exps[rc * p.exps_ld + cb / kAct8Block];
-        if (r >= end) eb = 0;                  // (a row that is none of this range's counts as zeros)
+        for (int q = 0; q < CP / 4; q++) x.b[q] = reinterpret_cast<const unsigned *>(p.codes + rc * p.codes_ld + cb)[q];
+        const unsigned e = p.exps[rc * p.exps_ld + cb / kAct8Block];
+        x.e = r < end ? e : 0u;
     };
-    auto stage = [&](unsigned char *s) {
+    auto stage = [&](unsigned char *s, Raw &x, auto with_sums) {
 #pragma unroll
         for (int v = 0; v < PA; v++) {
             unsigned h0, m0, l0, h1, m1, l1;
-            split3_pair(f32x2{xa[v][0], xa[v][1]}, h0, m0, l0);
-            split3_pair(f32x2{xa[v][2], xa[v][3]}, h1, m1, l1);
-            const int off = plane_off<TM>(ra + (1024 / TM) * v, (tid % LA) >> 1) + 8 * (tid & 1);
+            split3_pair(f32x2{x.a[v][0], x.a[v][1]}, h0, m0, l0);
+            split3_pair(f32x2{x.a[v][2], x.a[v][3]}, h1, m1, l1);
+            const int off = plane_off<TM>(ra + RA * v, (tid % LA) >> 1) + 8 * (tid & 1);
             *reinterpret_cast<u32x2 *>(s + off) = u32x2{h0, h1};
             *reinterpret_cast<u32x2 *>(s + kPlaneA + off) = u32x2{m0, m1};
             *reinterpret_cast<u32x2 *>(s + 2 * kPlaneA + off) = u32x2{l0, l1};
-            if (sums) colsum += xa[v];
+            if constexpr (decltype(with_sums)::value) colsum += x.a[v];
         }
-        const float step = act8_step(eb);
         unsigned char *b = s + 3 * kPlaneA;
+        const float step = act8_step((int)x.e);
+        unsigned o[CP / 2];
 #pragma unroll
-        for (int c = 0; c < CP / 8; c++) {
-            unsigned o[4];
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const unsigned w = act8_clear_marks(xb[2 * c + q]);
-                o[2 * q] = exact_bf16_pair(act8_value(w, 0, step), act8_value(w, 1, step));
-                o[2 * q + 1] = exact_bf16_pair(act8_value(w, 2, step), act8_value(w, 3, step));
-            }
-            *reinterpret_cast<u32x4 *>(b + plane_off<TN>(rb, (tid % LB) * (CP / 8) + c)) = u32x4{o[0], o[1], o[2], o[3]};
+        for (int q = 0; q < CP / 4; q++) {
+            const unsigned w = act8_clear_marks(x.b[q]);
+            o[2 * q] = exact_bf16_pair(act8_value(w, 0, step), act8_value(w, 1, step));
+            o[2 * q + 1] = exact_bf16_pair(act8_value(w, 2, step), act8_value(w, 3, step));
         }
+        if constexpr (CP == 4) *reinterpret_cast<u32x2 *>(b + plane_off<TN>(rb, (tid % LB) >> 1) + 8 * (tid & 1)) = u32x2{o[0], o[1]};
+        else
+#pragma unroll
+            for (int c = 0; c < CP / 8; c++)
+                *reinterpret_cast<u32x4 *>(b + plane_off<TN>(rb, (tid % LB) * (CP / 8) + c)) = u32x4{o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]};
     };
-    auto multiply = [&](const unsigned char *s) {
+    bf16x8 fa[MI][3], fb[NI];
+    auto fragments = [&](const unsigned char *s) {
 #pragma unroll
-        for (int sl = 0; sl < 2; sl++) {
-            bf16x8 a[MI][3], b[NI];
+        for (int ni = 0; ni < NI; ni++) fb[ni] = plane_frag<TN>(s + 3 * kPlaneA, wc * (TN / 2) + 32 * ni);
 #pragma unroll
-            for (int ni = 0; ni < NI; ni++) b[ni] = plane_frag<TN>(s + 3 * kPlaneA, wc * (TN / 2) + 32 * ni, sl);
+        for (int k = 2; k >= 0; k--)
+#pragma unroll
+            for (int mi = 0; mi < MI; mi++) fa[mi][k] = plane_frag<TM>(s + k * kPlaneA, wr * (TM / 2) + 32 * mi);
+    };
+    auto multiply = [&]() {
+#pragma unroll
+        for (int k = 2; k >= 0; k--)                // smallest terms first
 #pragma unroll
             for (int mi = 0; mi < MI; mi++)
 #pragma unroll
-                for (int k = 2; k >= 0; k--) a[mi][k] = plane_frag<TM>(s + k * kPlaneA, wr * (TM / 2) + 32 * mi, sl);
-#pragma unroll
-            for (int k = 2; k >= 0; k--)                // smallest terms first
-#pragma unroll
-                for (int mi = 0; mi < MI; mi++)
-#pragma unroll
-                    for (int ni = 0; ni < NI; ni++)
-                        acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[mi][k], b[ni], acc[mi][ni], 0, 0, 0);
-        }
+                for (int ni = 0; ni < NI; ni++)
+                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[mi][k], fb[ni], acc[mi][ni], 0, 0, 0);
     };
 
-    load(0);
-    stage(smem);
-    __syncthreads();
-    for (int t = 0; t < steps; t++) {
-        unsigned char *now = smem + (t & 1) * kStage, *next = smem + ((t + 1) & 1) * kStage;
-        if (t + 1 < steps) load(t + 1);
-        multiply(now);
-        if (t + 1 < steps) stage(next);
+    // Steps [t0, t1) by one way of requesting them.  During step t the operands of t + 2 are requested, those of t + 1 (which
+    // arrived meanwhile) converted and written to the other stage, and the MFMAs of t run.  Requests past the last step repeat it.
+    auto run = [&](auto whole, auto with_sums, int t0, int t1) {
+        auto get = [&](int t, Raw &x) {
+            if constexpr (decltype(whole)::value) request(min(t, t1 - 1), x);
+            else request_any(min(t, t1 - 1), x);
+        };
+        Raw u, w;
+        auto step = [&](int t, unsigned char *now, unsigned char *next, Raw &gone, Raw &come) {
+            get(t + 2, gone);
+            __builtin_amdgcn_sched_barrier(0);
+            fragments(now);
+#pragma unroll
+            for (int v = 0; v < PA; v++) pin(come.a[v]);
+#pragma unroll
+            for (int q = 0; q < CP / 4; q++) pin(come.b[q]);
+            pin(come.e);
+            stage(next, come, with_sums);
+            multiply();
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * (3 * MI + NI), 0);
+            interleave<0, 3 * MI * NI, 24 * PA + 4 * CP, 3 * PA + (CP + 7) / 8>();
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+        };
+        get(t0, u);
+        get(t0 + 1, w);
+        stage(smem, u, with_sums);
         __syncthreads();
-    }
+        int t = t0;
+        for (; t + 2 < t1; t += 2) {
+            step(t, smem, smem + kStage, u, w);
+            step(t + 1, smem + kStage, smem, w, u);
+        }
+        if (t + 1 < t1) {
+            step(t, smem, smem + kStage, u, w);
+            fragments(smem + kStage);
+        } else fragments(smem);
+        multiply();
+        __syncthreads();
+    };
+    auto run_all = [&](auto with_sums) {
+        const int fast = p.dz_vec ? full : 0;
+        if (fast > 0) run(std::true_type{}, with_sums, 0, fast);
+        if (fast < steps) run(std::false_type{}, with_sums, fast, steps);
+    };
+    if (sums) run_all(std::true_type{});
+    else run_all(std::false_type{});
 
     if (sums) {         // this thread's four columns over its rows -> the tile's, in a fixed order
         float *meet = reinterpret_cast<float *>(smem);
@@ -205,14 +273,45 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
         }
 }
 
+// Tile and ranges.  The widest tile that still gives 256 workgroups with at least 512 rows each is taken, cut into ranges
+// until there are 512 workgroups (two per compute unit, measured below against one and four); what is smaller gets 64 x 64
+// tiles and 256 workgroups.  Measured (us; tile, workgroups): 65536 x 1024 x 1024 339 (128x256, 512), 409 (256), 361 (1024),
+// 407 (128x128, 512); 8192 x 512 x 1024 39.3 (128x256, 256), 41.4 (64x128, 768); 8192 x 256 x 512 22.2 (64x128, 256),
+// 24.6 (128x128, 256); 8192 x 128 x 256 12.2 (64x64, 256), 13.9 (128x64, 256); 512 x 1024 x 1024 12.8 (64x64, 256), 17.3 (512).
+Wgrad8Shape wgrad8_shape(int64_t M, int N, int K, size_t max_bytes) {
+    static const struct { int tm, tn; int64_t want, depth; } tiles[4] = {{128, 256, 512, 512}, {128, 128, 512, 512}, {64, 128, 512, 512}, {64, 64, 256, 256}};
+    int64_t s = 1;
+    int pick = 3;
+    for (int i = 0; i < 4; i++) {
+        const int64_t n = ceil_div(N, tiles[i].tm) * ceil_div(K, tiles[i].tn);
+        s = ceil_div(tiles[i].want, n);
+        s = s > M / tiles[i].depth ? M / tiles[i].depth : s;
+        s = s < 1 ? 1 : (s > 256 ? 256 : s);
+        pick = i;
+        // (a tile that N or K fills to no more than half leaves the other half of its work to columns that do not exist)
+        if (n * s >= 256 && (tiles[i].tm == 64 || 2 * N > tiles[i].tm) && (tiles[i].tn == 64 || 2 * K > tiles[i].tn)) break;
+    }
+    const size_t slab = sizeof(float) * ((size_t)N * K + N);
+    if (max_bytes != 0 && (size_t)s * slab > max_bytes) s = max_bytes < 2 * slab ? 1 : (int64_t)(max_bytes / slab);
+    Wgrad8Shape w{};
+    w.tm = tiles[pick].tm;
+    w.tn = tiles[pick].tn;
+    const int64_t rows = ceil_div(ceil_div(M < 1 ? 1 : M, s), 32) * 32;
+    w.rows_per_split = (int)rows;
+    w.splits = (int)ceil_div(M < 1 ? 1 : M, rows);
+    w.bytes = w.splits * slab + 256;
+    return w;
+}
+
 int launch_wgrad8(Wgrad8 p, int tm, int tn, hipStream_t s) {
     p.gx = (int)ceil_div(p.K, tn);
     p.gy = (int)ceil_div(p.N, tm);
     const int64_t nwg = (int64_t)p.gx * p.gy * p.gz;
     DLRM_REQUIRE(nwg < (1ll << 31), "GEMM grid too large");
+    DLRM_REQUIRE(p.dz_ld <= (1 << 24) && p.codes_ld <= (1 << 24) && p.exps_ld <= (1 << 24), "leading dimension above 2^24");
     const dim3 grid((unsigned)nwg), block(256);
-    if (tm == 128 && tn == 128) hipLaunchKernelGGL((wgrad8_kernel<128, 128>), grid, block, 0, s, p);
-    else if (tm == 128) hipLaunchKernelGGL((wgrad8_kernel<128, 64>), grid, block, 0, s, p);
+    if (tn == 256) hipLaunchKernelGGL((wgrad8_kernel<128, 256>), grid, block, 0, s, p);
+    else if (tm == 128) hipLaunchKernelGGL((wgrad8_kernel<128, 128>), grid, block, 0, s, p);
     else if (tn == 128) hipLaunchKernelGGL((wgrad8_kernel<64, 128>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((wgrad8_kernel<64, 64>), grid, block, 0, s, p);
     DLRM_LAUNCH_CHECK();

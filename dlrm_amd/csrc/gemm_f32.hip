@@ -1973,8 +1973,15 @@ extern "C" int dlrm_linear_backward_weight_workspace_bytes(int64_t M, int32_t N,
     return DLRM_OK;
 }
 
+extern "C" int dlrm_linear_backward_weight_act8_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t *bytes) {
+    DLRM_REQUIRE(bytes != nullptr && M >= 0 && N >= 1 && K >= 1, "bad arguments");
+    *bytes = wgrad8_shape(M, N, K, 0).bytes;
+    return DLRM_OK;
+}
+
+// max_bytes != 0: the workspace is what it is, and a product from a checkpoint is cut into as many ranges as fit
 static int backward_weight_impl(const dlrm_linear_bwd *l, void *d_workspace, size_t workspace_bytes,
-                                dlrm_stream_t stream, SlabReduce *pending = nullptr) {
+                                dlrm_stream_t stream, SlabReduce *pending = nullptr, size_t max_bytes = 0) {
     if (pending) pending->splits = 0;
     DLRM_REQUIRE(l != nullptr, "linear_bwd descriptor is NULL");
     DLRM_REQUIRE(l->M >= 1 && l->N >= 1 && l->K >= 1, "bad shape");
@@ -1986,13 +1993,13 @@ static int backward_weight_impl(const dlrm_linear_bwd *l, void *d_workspace, siz
     if (from8)
         if (int rc = act8_check(&l->x8, l->K, "checkpoint of x")) return rc;
     size_t need = 0;
-    dlrm_linear_backward_weight_workspace_bytes(l->M, l->N, l->K, &need);
+    if (from8) need = max_bytes != 0 ? 0 : wgrad8_shape(l->M, l->N, l->K, 0).bytes;
+    else dlrm_linear_backward_weight_workspace_bytes(l->M, l->N, l->K, &need);
     DLRM_REQUIRE(d_workspace != nullptr && workspace_bytes >= need, "workspace too small: %zu < %zu", workspace_bytes,
                  need);
     DLRM_REQUIRE(aligned16(d_workspace), "workspace must be 16-byte aligned");
     hipStream_t s = as_stream(stream);
     int splits = 1;
-    const TileShape ts = wgrad_shape(l->M, l->N, l->K, from8 ? DLRM_GEMM_BF16X3 : l->gemm_mode, &splits);
     float *slabs = static_cast<float *>(d_workspace);
     if (from8) {
         Wgrad8 w{};
@@ -2000,15 +2007,17 @@ static int backward_weight_impl(const dlrm_linear_bwd *l, void *d_workspace, siz
         w.codes = l->x8.d_codes; w.codes_ld = l->x8.ld; w.exps = l->x8.d_exps; w.exps_ld = l->x8.exps_ld;
         w.blocks = act8_blocks(l->K);
         w.M = (int)l->M; w.N = l->N; w.K = l->K;
-        w.rows_per_split = (int)ceil_div(ceil_div(l->M, splits), BK) * BK;
-        w.gz = (int)ceil_div(l->M, w.rows_per_split);
-        float *db_slabs = slabs + (size_t)splits * l->N * l->K;
+        const Wgrad8Shape t = wgrad8_shape(l->M, l->N, l->K, max_bytes);
+        w.rows_per_split = t.rows_per_split;
+        w.gz = t.splits;
+        float *db_slabs = slabs + (size_t)w.gz * l->N * l->K;
         const bool whole = w.gz == 1;
         w.C = whole ? l->d_dw : slabs; w.ldc = whole ? l->dw_ld : l->K; w.slab_stride = (int64_t)l->N * l->K;
         w.colsum = l->d_db == nullptr ? nullptr : (whole ? l->d_db : db_slabs);
-        if (int rc = launch_wgrad8(w, ts.tm, ts.tn, s)) return rc;
+        if (int rc = launch_wgrad8(w, t.tm, t.tn, s)) return rc;
         return whole ? DLRM_OK : launch_reduce(slabs, w.slab_stride, l->N, l->K, l->d_dw, l->dw_ld, db_slabs, l->d_db, w.gz, s, pending);
     }
+    const TileShape ts = wgrad_shape(l->M, l->N, l->K, l->gemm_mode, &splits);
     const bool few_inputs = skinny_k_forward_ok(l->N, l->K);
     if (few_inputs || (l->N == 1 && gemv_backward_weight_ok(l->d_x, l->x_ld, l->K))) {
         // partial sums over row ranges, then the same fixed-order reduction as the split-batch product
@@ -2084,13 +2093,13 @@ extern "C" int dlrm_linear_backward_weight_static(const dlrm_linear_bwd *l, dlrm
     DLRM_REQUIRE(l->M >= 1 && l->N >= 1 && l->K >= 1, "bad shape");
     size_t need = 0;
     if (int rc = dlrm_linear_backward_weight_workspace_bytes(l->M, l->N, l->K, &need)) return rc;
-    DLRM_REQUIRE(need <= (size_t)DLRM_STATIC_SCRATCH_BYTES,
+    DLRM_REQUIRE(l->x8.d_codes != nullptr || need <= (size_t)DLRM_STATIC_SCRATCH_BYTES,
                  "layer M=%lld N=%d K=%d needs %zu bytes of partial sums, the static scratch holds %zu: use "
                  "dlrm_linear_backward_weight with a workspace", (long long)l->M, l->N, l->K, need,
                  (size_t)DLRM_STATIC_SCRATCH_BYTES);
     void *ws = nullptr;
     if (int rc = static_scratch(&ws)) return rc;
-    return backward_weight_impl(l, ws, (size_t)DLRM_STATIC_SCRATCH_BYTES, stream);
+    return backward_weight_impl(l, ws, (size_t)DLRM_STATIC_SCRATCH_BYTES, stream, nullptr, (size_t)DLRM_STATIC_SCRATCH_BYTES);
 }
 
 extern "C" int dlrm_sgd_step(float *d_w, const float *d_g, int64_t n, float lr, dlrm_stream_t stream) {

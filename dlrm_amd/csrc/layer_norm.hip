@@ -52,33 +52,36 @@ struct NormBwd {
     int N;
 };
 
-// sum over the TEAM lanes that share a row, the same bits in all of them.  Teams of several waves meet in `slot` (TEAM / 64
-// floats): the caller alternates between slots, so that a slot is written again only behind a later barrier.
+// sum over the TEAM lanes that share a row, the same bits in all of them.  Teams of several waves meet in `slot` (a float
+// for each wave of the workgroup): the caller alternates between slots, so that a slot is written again only behind a later barrier.
 template <int TEAM>
 __device__ inline float team_sum(float x, float *slot) {
     if constexpr (TEAM <= 64) return group_sum<TEAM>(x);
     else {
+        constexpr int W = TEAM / 64;
+        slot += threadIdx.x / TEAM * W;
         x = group_sum<64>(x);
-        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+        if ((threadIdx.x & 63) == 0) slot[(threadIdx.x >> 6) % W] = x;
         __syncthreads();
         float t = slot[0];
 #pragma unroll
-        for (int w = 1; w < TEAM / 64; w++) t += slot[w];
+        for (int w = 1; w < W; w++) t += slot[w];
         return t;
     }
 }
 template <int TEAM>
-__device__ inline void team_sum2(float &x, float &y, float *slot) {     // slot: 2 TEAM / 64 floats
+__device__ inline void team_sum2(float &x, float &y, float *slot) {     // slot: two floats a wave
     if constexpr (TEAM <= 64) {
         x = group_sum<TEAM>(x);
         y = group_sum<TEAM>(y);
     } else {
         constexpr int W = TEAM / 64;
+        slot += threadIdx.x / TEAM * 2 * W;
         x = group_sum<64>(x);
         y = group_sum<64>(y);
         if ((threadIdx.x & 63) == 0) {
-            slot[threadIdx.x >> 6] = x;
-            slot[W + (threadIdx.x >> 6)] = y;
+            slot[(threadIdx.x >> 6) % W] = x;
+            slot[W + (threadIdx.x >> 6) % W] = y;
         }
         __syncthreads();
         x = slot[0];
@@ -150,7 +153,7 @@ __device__ inline void norm_output(const NormFwd &p, int64_t row, int c, bool li
 template <typename T, int V, int TEAM>
 __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(NormFwd p) {
     constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
-    __shared__ float slots[2][TEAM > 64 ? TEAM / 64 : 1];
+    __shared__ float slots[2][TEAM > 64 ? kThreads / 64 : 1];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     float g[V][VEC], b[V][VEC];
 #pragma unroll
@@ -292,13 +295,14 @@ struct NormGradPiece {
 template <typename T, int V, int TEAM, bool FROM8, int MASK>
 __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(NormBwd p) {
     constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
-    __shared__ float slots[2][TEAM > 64 ? TEAM / 32 : 1];
+    __shared__ float slots[2][TEAM > 64 ? kThreads / 32 : 1];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    constexpr bool kHoldGamma = TEAM < 512;     // (workgroups of 8 waves and more have no registers for it: read again per row)
     float g[V][VEC], acc_g[V][VEC], acc_b[V][VEC];
 #pragma unroll
     for (int v = 0; v < V; v++) {
         const int c = (v * TEAM + lane) * VEC;
-        param_elems<VEC>(p.gamma, c, p.N, g[v], 1.f);
+        if (kHoldGamma) param_elems<VEC>(p.gamma, c, p.N, g[v], 1.f);
 #pragma unroll
         for (int j = 0; j < VEC; j++) acc_g[v][j] = acc_b[v][j] = 0.f;
     }
@@ -315,7 +319,8 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
 #pragma unroll
         for (int v = 0; v < V; v++) piece[v].values(p, (v * TEAM + lane) * VEC, mean, rstd, xh[v], d[v]);
 #pragma unroll
-        for (int v = 0; v < V; v++)
+        for (int v = 0; v < V; v++) {
+            if (!kHoldGamma) param_elems<VEC>(p.gamma, (v * TEAM + lane) * VEC, p.N, g[v], 1.f);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 if (live) {
@@ -326,6 +331,7 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
                 s1 += d[v][j];
                 s2 = __builtin_fmaf(d[v][j], xh[v][j], s2);
             }
+        }
         team_sum2<TEAM>(s1, s2, slots[turn]);
         const float c1 = s1 / (float)p.N, c2 = s2 / (float)p.N;
 #pragma unroll
@@ -481,7 +487,7 @@ static int64_t norm_bwd_parts(int64_t M, int N) {       // most partial rows tha
 template <typename T, int V, int TEAM>
 static void launch_fwd(const NormFwd &p, hipStream_t s) {
     constexpr int kThreads = TEAM > 256 ? TEAM : 256;
-    const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = TEAM > 256 ? 512 : 2048;
+    const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = 2048 / (kThreads / 256);
     hipLaunchKernelGGL((norm_fwd_kernel<T, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
 }
 
@@ -538,7 +544,8 @@ static void launch_bwd_long(NormBwd p, float *dgamma, float *dbeta, int64_t *par
     }
 }
 
-// one team shape per width: the smallest that holds the row
+// One team shape per width: the smallest that holds the row with up to 16 float32 or 8 bf16 elements a lane.  More elements
+// cost registers and with them waves in flight: bf16 backward 65536 x 1024 from x 168 us with 16 a lane, 104 us with 8.
 #define DLRM_NORM_SHAPES(T, N, CALL, LONG, ...)                                \
     do {                                                                       \
         constexpr int W = kWide<T>, F = W / 4;                                 \
@@ -546,11 +553,11 @@ static void launch_bwd_long(NormBwd p, float *dgamma, float *dbeta, int64_t *par
         else if ((N) <= 16 * W) CALL<T, 1, 16>(__VA_ARGS__);                   \
         else if ((N) <= 32 * W) CALL<T, 1, 32>(__VA_ARGS__);                   \
         else if ((N) <= 64 * W) CALL<T, 1, 64>(__VA_ARGS__);                   \
-        else if ((N) <= 512 * F) CALL<T, 2, 64>(__VA_ARGS__);                  \
-        else if ((N) <= 1024 * F) CALL<T, 4, 64>(__VA_ARGS__);                 \
-        else if ((N) <= 2048) CALL<T, 8 / F, 64>(__VA_ARGS__);                 \
-        else if ((N) <= 4096) CALL<T, 4 / F, 256>(__VA_ARGS__);                \
-        else if ((N) <= 8192) CALL<T, 8 / F, 256>(__VA_ARGS__);                \
+        else if ((N) <= 512) CALL<T, 2 / F, 64>(__VA_ARGS__);                  \
+        else if ((N) <= 1024) CALL<T, 4 / (F * F), 64 * F>(__VA_ARGS__);       \
+        else if ((N) <= 2048) CALL<T, 4 / (F * F), 128 * F>(__VA_ARGS__);      \
+        else if ((N) <= 4096) CALL<T, 4 / (F * F), 256 * F>(__VA_ARGS__);      \
+        else if ((N) <= 8192) CALL<T, 4 / (F * F), 512 * F>(__VA_ARGS__);      \
         else if ((N) <= kLongRow) CALL<T, 4 / F, 1024>(__VA_ARGS__);           \
         else LONG<T>(__VA_ARGS__);                                             \
     } while (0)

@@ -506,9 +506,12 @@ def absmax_(x, slot):
 
 
 @functools.lru_cache(maxsize=4096)
-def linear_backward_weight_workspace_bytes(M, N, K):
+def linear_backward_weight_workspace_bytes(M, N, K, act8=False):
+    """act8: for a weight gradient from an Act8."""
     n = C.c_size_t(0)
-    check(_capi.lib().dlrm_linear_backward_weight_workspace_bytes(C.c_int64(M), N, K, C.byref(n)))
+    L = _capi.lib()
+    query = L.dlrm_linear_backward_weight_act8_workspace_bytes if act8 else L.dlrm_linear_backward_weight_workspace_bytes
+    check(query(C.c_int64(M), N, K, C.byref(n)))
     return int(n.value)
 
 
@@ -525,7 +528,7 @@ def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True
         dw = torch.empty((N, K), dtype=torch.float32, device=dz.device)
     if db is None and want_db:
         db = torch.empty((N,), dtype=torch.float32, device=dz.device)
-    need = linear_backward_weight_workspace_bytes(M, N, K)
+    need = linear_backward_weight_workspace_bytes(M, N, K, x8 is not None)
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dz.device)
     d = _capi.LinearBwdDesc()

@@ -353,6 +353,8 @@ typedef struct dlrm_linear_bwd {
 
 int dlrm_linear_backward_data(const dlrm_linear_bwd *l, dlrm_stream_t stream);
 int dlrm_linear_backward_weight_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t *bytes);
+/* The same query for a weight gradient from x8. */
+int dlrm_linear_backward_weight_act8_workspace_bytes(int64_t M, int32_t N, int32_t K, size_t *bytes);
 int dlrm_linear_backward_weight(const dlrm_linear_bwd *l, void *d_workspace, size_t workspace_bytes,
                                 dlrm_stream_t stream);
 /*
@@ -366,6 +368,8 @@ int dlrm_linear_backward_weight(const dlrm_linear_bwd *l, void *d_workspace, siz
  * layer of the Criteo-Kaggle and MLPerf models fits, at any batch).  All calls on one GPU share the array:
  * calls that overlap in time on one GPU (two streams, two threads) race; calls on one stream do not.
  * Nothing in the array has to be zero between calls: every partial sum that is read was written by the same call.
+ * A weight gradient from x8 is never refused for its size: its batch is cut into as many ranges as the array holds
+ * partial sums for (down to one, which needs none), so beyond 40 MB of them its sums are grouped differently.
  */
 #define DLRM_STATIC_SCRATCH_BYTES (40u << 20)
 int dlrm_linear_backward_weight_static(const dlrm_linear_bwd *l, dlrm_stream_t stream);

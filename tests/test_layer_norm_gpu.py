@@ -256,7 +256,7 @@ def test_graph_replays():
                dx=torch.empty((M, N), device="cuda"), dg=torch.empty(N, device="cuda"), db=torch.empty(N, device="cuda"),
                dw=torch.empty((N, K), device="cuda"), dwb=torch.empty(N, device="cuda"))
     ws1 = torch.empty(ops.layer_norm_backward_workspace_bytes(M, N), dtype=torch.uint8, device="cuda")
-    ws2 = torch.empty(ops.linear_backward_weight_workspace_bytes(M, N, K), dtype=torch.uint8, device="cuda")
+    ws2 = torch.empty(ops.linear_backward_weight_workspace_bytes(M, N, K, True), dtype=torch.uint8, device="cuda")
 
     def step():
         ops.act8_pack(sin, out=in8)
