@@ -27,7 +27,6 @@ int act8_check(const dlrm_act8 *a, int cols, const char *what);
 struct Wgrad8 {
     const float *dz;
     int64_t dz_ld;
-    int dz_vec;              // rows of dz start on 16-byte boundaries
     const int8_t *codes;
     int64_t codes_ld;
     const uint8_t *exps;

@@ -21,6 +21,7 @@ namespace dlrm {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4u __attribute__((aligned(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -71,7 +72,8 @@ __device__ inline unsigned exact_bf16_pair(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
-template <int TM, int TN>
+// CUT: N is no multiple of four, so the last tile along it has pieces that N cuts through
+template <int TM, int TN, bool CUT>
 __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     constexpr int MI = TM / 64, NI = TN / 64;
     constexpr int PA = TM / 64, LA = TM / 4, RA = 256 / LA;     // dz: 16-byte pieces per thread and step, lanes per row, rows per piece
@@ -90,9 +92,9 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     const int begin = bz * p.rows_per_split, end = min(p.M, begin + p.rows_per_split);
     const int full = (end - begin) / kStepRows, steps = (end - begin + kStepRows - 1) / kStepRows;
 
-    // columns past the operands only feed outputs that are never stored: their loads are moved inside the row
-    int ca = n0 + 4 * (tid % LA);
-    if (p.dz_vec && ca + 4 > p.dz_ld) ca = (int)p.dz_ld - 4;
+    // Columns past the operands only feed outputs that are never stored: their loads are moved inside the row.  A piece of dz
+    // that N cuts through is moved back too and put in its place in registers.
+    const int ca = n0 + 4 * (tid % LA), ca_in = max(min(ca, p.N - 4), 0), shift = ca < p.N ? ca - ca_in : 0;
     const int ra = tid / LA;
     int cb = k0 + CP * (tid % LB);
     if (cb + CP > p.blocks * kAct8Block) cb = p.blocks * kAct8Block - CP;
@@ -113,14 +115,14 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
         unsigned b[CP / 4], e;
     };
     // a wave-uniform origin and 32-bit offsets that no step changes (the launch bounds the row lengths)
-    const unsigned oa = ((unsigned)ra * (unsigned)p.dz_ld + (unsigned)ca) * 4u, ob = (unsigned)rb * (unsigned)p.codes_ld + (unsigned)cb;
+    const unsigned oa = ((unsigned)ra * (unsigned)p.dz_ld + (unsigned)ca_in) * 4u, ob = (unsigned)rb * (unsigned)p.codes_ld + (unsigned)cb;
     const unsigned oe = (unsigned)rb * (unsigned)p.exps_ld + (unsigned)(cb / kAct8Block);
-    auto request = [&](int t, Raw &x) {       // a whole step on 16-byte boundaries
+    auto request = [&](int t, Raw &x) {       // a whole step of rows of at least four (16-byte loads at any alignment)
         const int64_t r0 = begin + t * kStepRows;
         const char *a = reinterpret_cast<const char *>(p.dz + r0 * p.dz_ld);
         const int8_t *b = p.codes + r0 * p.codes_ld;
 #pragma unroll
-        for (int v = 0; v < PA; v++) x.a[v] = *reinterpret_cast<const f32x4 *>(a + (oa + (unsigned)(RA * v) * (unsigned)p.dz_ld * 4u));
+        for (int v = 0; v < PA; v++) x.a[v] = *reinterpret_cast<const f32x4u *>(a + (oa + (unsigned)(RA * v) * (unsigned)p.dz_ld * 4u));
         if constexpr (CP == 16) {
             const u32x4 w = *reinterpret_cast<const u32x4 *>(b + ob);
 #pragma unroll
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
             const float *row = p.dz + (int64_t)min(r, end - 1) * p.dz_ld;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const float f = row[p.dz_vec ? ca + q : min(ca + q, p.N - 1)];
+                const float f = row[min(ca + q, p.N - 1)];
                 x.a[v][q] = r < end ? f : 0.f;
             }
         }
@@ -200,9 +202,20 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     // Steps [t0, t1) by one way of requesting them.  During step t the operands of t + 2 are requested, those of t + 1 (which
     // arrived meanwhile) converted and written to the other stage, and the MFMAs of t run.  Requests past the last step repeat it.
     auto run = [&](auto whole, auto with_sums, int t0, int t1) {
+        constexpr bool kWhole = decltype(whole)::value;
         auto get = [&](int t, Raw &x) {
-            if constexpr (decltype(whole)::value) request(min(t, t1 - 1), x);
+            if constexpr (kWhole) request(min(t, t1 - 1), x);
             else request_any(min(t, t1 - 1), x);
+        };
+        auto place = [&](Raw &x) {
+            if constexpr (kWhole && CUT)
+#pragma unroll
+                for (int v = 0; v < PA; v++) {
+                    f32x4 a = x.a[v];
+                    if (shift & 1) a = f32x4{a[1], a[2], a[3], a[3]};
+                    if (shift & 2) a = f32x4{a[2], a[3], a[3], a[3]};
+                    x.a[v] = a;
+                }
         };
         Raw u, w;
         auto step = [&](int t, unsigned char *now, unsigned char *next, Raw &gone, Raw &come) {
@@ -214,6 +227,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
 #pragma unroll
             for (int q = 0; q < CP / 4; q++) pin(come.b[q]);
             pin(come.e);
+            place(come);
             stage(next, come, with_sums);
             multiply();
             __builtin_amdgcn_sched_group_barrier(0x100, 2 * (3 * MI + NI), 0);
@@ -223,6 +237,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
         };
         get(t0, u);
         get(t0 + 1, w);
+        place(u);
         stage(smem, u, with_sums);
         __syncthreads();
         int t = t0;
@@ -238,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
         __syncthreads();
     };
     auto run_all = [&](auto with_sums) {
-        const int fast = p.dz_vec ? full : 0;
+        const int fast = p.N >= 4 ? full : 0;
         if (fast > 0) run(std::true_type{}, with_sums, 0, fast);
         if (fast < steps) run(std::false_type{}, with_sums, fast, steps);
     };
@@ -310,10 +325,16 @@ int launch_wgrad8(Wgrad8 p, int tm, int tn, hipStream_t s) {
     DLRM_REQUIRE(nwg < (1ll << 31), "GEMM grid too large");
     DLRM_REQUIRE(p.dz_ld <= (1 << 24) && p.codes_ld <= (1 << 24) && p.exps_ld <= (1 << 24), "leading dimension above 2^24");
     const dim3 grid((unsigned)nwg), block(256);
-    if (tn == 256) hipLaunchKernelGGL((wgrad8_kernel<128, 256>), grid, block, 0, s, p);
-    else if (tm == 128) hipLaunchKernelGGL((wgrad8_kernel<128, 128>), grid, block, 0, s, p);
-    else if (tn == 128) hipLaunchKernelGGL((wgrad8_kernel<64, 128>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((wgrad8_kernel<64, 64>), grid, block, 0, s, p);
+#define DLRM_WGRAD8(TM, TN)                                                                                   \
+    do {                                                                                                      \
+        if (p.N % 4 == 0) hipLaunchKernelGGL((wgrad8_kernel<TM, TN, false>), grid, block, 0, s, p);           \
+        else hipLaunchKernelGGL((wgrad8_kernel<TM, TN, true>), grid, block, 0, s, p);                         \
+    } while (0)
+    if (tn == 256) DLRM_WGRAD8(128, 256);
+    else if (tm == 128) DLRM_WGRAD8(128, 128);
+    else if (tn == 128) DLRM_WGRAD8(64, 128);
+    else DLRM_WGRAD8(64, 64);
+#undef DLRM_WGRAD8
     DLRM_LAUNCH_CHECK();
     return DLRM_OK;
 }

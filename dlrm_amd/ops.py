@@ -15,7 +15,7 @@ from ._capi import (BF16, F32, I32, I64, EmbBagDesc, SparseOpt, check)  # noqa: 
 
 def _stream():
     # (the raw handle: building the Stream object around it costs more than the rest of a small launch's Python)
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 # While a StepRecorder is installed (dlrm_amd.plan), the operators below do everything except launch:
@@ -24,11 +24,18 @@ _recorder = None
 _gemm_mode = {"0": 0, "1": 1, "2": 2}.get(os.environ.get("DLRM_GEMM_MODE", "1").strip(), 1)
 
 
+_entries = {}      # entry points by operator name
+
+
 def _emit(name, *args):
     """Launch `dlrm_<name>(*args, stream)` now, or record it."""
     if _recorder is None:
-        args = [C.byref(a) if isinstance(a, C.Structure) else a for a in args]
-        check(getattr(_capi.lib(), "dlrm_" + name)(*args, _stream()))
+        fn = _entries.get(name)
+        if fn is None:
+            fn = _entries[name] = getattr(_capi.lib(), "dlrm_" + name)
+        rc = fn(*[C.byref(a) if isinstance(a, C.Structure) else a for a in args], _stream())
+        if rc:
+            check(rc)
     else:
         _recorder.add(name, args)
 

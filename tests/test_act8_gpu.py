@@ -156,6 +156,21 @@ def test_data_gradient_with_weight_planes():
         ops.set_gemm_mode(old)
 
 
+@pytest.mark.parametrize("M,N,K", [(9300, 520, 700), (9300, 518, 701), (22100, 300, 200), (22101, 299, 193), (32800, 60, 500),
+                                   (32811, 59, 499)])
+def test_weight_gradient_of_every_tile(M, N, K):
+    """Batches that give the wide tiles enough row ranges (of up to 576 rows): 3 * 36 matrix additions a range, at most 64 ranges
+    here, so 180 U sum |dz x|."""
+    from dlrm_amd import ops
+    _, a, x = checkpoint(M, K)
+    g = torch.Generator().manual_seed(M + N)
+    dz = torch.randn(M, N, generator=g) * torch.exp(2 * torch.randn(M, 1, generator=g))
+    dw, db, _ = ops.linear_backward_weight(dz.cuda(), a)
+    want = dz.double().t() @ x
+    assert ((dw.cpu().double() - want).abs() <= 180 * U * (dz.double().abs().t() @ x.abs())).all()
+    assert ((db.cpu().double() - dz.double().sum(0)).abs() <= 180 * U * dz.double().abs().sum(0)).all()
+
+
 def test_weight_gradient_of_wide_values():
     """Columns and samples many decades apart, blocks of zeros, a block that holds a NaN: its columns alone see it."""
     from dlrm_amd import ops
