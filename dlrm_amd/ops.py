@@ -208,35 +208,43 @@ def embbag_backward_apply(weight, indices, offsets, batch, grad, workspace, num_
 # ------------------------------------------- 8-bit activation checkpoints
 
 
-def _require_here(*ts):
-    """Device tensors of the current device (the launch goes to its current stream)."""
-    here = None
-    for t in ts:
-        if t is not None:
-            at = t.get_device()
-            if at != here:
-                if at < 0:
-                    raise _capi.DlrmError("dlrm_amd ops need device tensors (there is no CPU fallback)")
-                here = torch.cuda.current_device()
-                if at != here:
-                    raise _capi.DlrmError("a tensor lives on cuda:%d, the current device is cuda:%d" % (at, here))
+# (A small call costs more host time than GPU time, most of it in questions to tensors: the helpers below ask each once.)
 
 
-def _rows(t, what, shape=None):
-    """Leading dimension of a [rows, cols] tensor whose rows are contiguous."""
+def _elsewhere(t):
+    if not t.is_cuda:
+        raise _capi.DlrmError("dlrm_amd ops need device tensors (there is no CPU fallback)")
+    raise _capi.DlrmError("a tensor lives on cuda:%d, the current device is cuda:%d"
+                          % (t.get_device(), torch.cuda.current_device()))
+
+
+def _device_of(t):
+    """The device of a call's first operand, which must be the current one (the launch goes to its current stream)."""
+    at = t.get_device()
+    if at < 0 or at != torch._C._cuda_getDevice():
+        _elsewhere(t)
+    return at
+
+
+def _rows(t, what, here, shape=None):
+    """Leading dimension of a [rows, cols] tensor on device `here` whose rows are contiguous."""
     s, st = t.shape, t.stride()
     if len(s) != 2 or (st[1] != 1 and s[1] > 1) or (shape is not None and s != shape):
         raise ValueError("%s must be a row-major [rows, cols] tensor%s, got shape %s and strides %s"
                          % (what, "" if shape is None else " of shape %s" % (tuple(shape),), tuple(s), st))
+    if t.get_device() != here:
+        _elsewhere(t)
     return st[0] if s[0] > 1 else max(st[0], s[1])
 
 
-def _vector(t, n, what):
-    """Address of a contiguous float32 [n] tensor (0 for None)."""
+def _vector(t, n, what, here):
+    """Address of a contiguous float32 [n] tensor on device `here` (0 for None)."""
     if t is None:
         return 0
     if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError("%s must be a contiguous float32 tensor of %d elements, got %s %s" % (what, n, t.dtype, tuple(t.shape)))
+    if t.get_device() != here:
+        _elsewhere(t)
     return t.data_ptr()
 
 
@@ -255,25 +263,26 @@ class Act8:
     Goes wherever the backward pass takes the activation it stands for: linear_backward_weight's x, linear_backward_data's and
     layer_norm_backward's relu_mask, and (made of the normalised rows by layer_norm_forward) layer_norm_backward's x."""
 
-    __slots__ = ("codes", "exps", "cols", "shape", "desc")
+    __slots__ = ("codes", "exps", "cols", "shape", "device_index", "desc")
 
     def __init__(self, codes, exps, cols):
         if codes.dtype is not torch.int8 or exps.dtype is not torch.uint8:
             raise TypeError("codes must be int8 and exponents uint8, got %s and %s" % (codes.dtype, exps.dtype))
         blocks = (cols + 31) // 32
-        ld, exps_ld = _rows(codes, "codes"), _rows(exps, "exponents")
-        rows, width = codes.shape
-        if cols < 1 or exps.shape[0] != rows or width < 32 * blocks or exps.shape[1] < blocks:
+        here = codes.get_device()
+        ld, exps_ld = _rows(codes, "codes", here), _rows(exps, "exponents", exps.get_device())
+        (rows, width), (exp_rows, exp_width) = codes.shape, exps.shape
+        if cols < 1 or exp_rows != rows or width < 32 * blocks or exp_width < blocks:
             raise ValueError("%d columns need codes [rows, %d] and exponents [rows, %d], got %s and %s"
                              % (cols, 32 * blocks, blocks, tuple(codes.shape), tuple(exps.shape)))
-        if codes.get_device() != exps.get_device():
+        if exps.get_device() != here:
             raise ValueError("codes and exponents live on different devices")
         if rows == 1:
             ld = (ld + 15) // 16 * 16
         at = codes.data_ptr()
         if ld % 16 or at % 16:
             raise ValueError("rows of codes must start on 16-byte boundaries")
-        self.codes, self.exps, self.cols, self.shape = codes, exps, cols, torch.Size((rows, cols))
+        self.codes, self.exps, self.cols, self.shape, self.device_index = codes, exps, cols, (rows, cols), here
         self.desc = _capi.Act8Desc(at, ld, exps.data_ptr(), exps_ld)
 
     @staticmethod
@@ -286,30 +295,29 @@ class Act8:
 _no_act8 = _capi.Act8Desc()
 
 
-def _act8(a, shape, what):
-    """Descriptor of a checkpoint that must have this shape (None: an empty one).  The caller has checked its device."""
+def _act8(a, shape, what, here):
+    """Descriptor of a checkpoint on device `here` that must have this shape (None: an empty one)."""
     if a is None:
         return _no_act8
     if not isinstance(a, Act8):
         raise TypeError("%s must be an Act8, got %s" % (what, type(a).__name__))
     if a.shape != shape:
-        raise ValueError("%s is a checkpoint of shape %s, expected %s" % (what, tuple(a.shape), tuple(shape)))
+        raise ValueError("%s is a checkpoint of shape %s, expected %s" % (what, a.shape, tuple(shape)))
+    if a.device_index != here:
+        _elsewhere(a.codes)
     return a.desc
-
-
-def _codes(a):
-    return a.codes if isinstance(a, Act8) else a
 
 
 @_op
 def act8_pack(x, out=None):
     """The 8-bit checkpoint of a float32 or bf16 activation [rows, cols] (rows may be strided)."""
-    ld = _rows(x, "x")
-    _require_here(x, None if out is None else out.codes)
+    here = _device_of(x)
+    ld = _rows(x, "x", here)
+    rows, cols = shape = x.shape
     if out is None:
-        out = Act8.empty(x.shape[0], x.shape[1], x.device)
-    d = _act8(out, x.shape, "out")
-    _emit("act8_pack", _ptr(x), C.c_int32(_act_dtype(x, "x")), C.c_int64(x.shape[0]), C.c_int32(x.shape[1]), C.c_int64(ld), d)
+        out = Act8.empty(rows, cols, x.device)
+    _emit("act8_pack", C.c_void_p(x.data_ptr()), C.c_int32(_act_dtype(x, "x")), C.c_int64(rows), C.c_int32(cols), C.c_int64(ld),
+          _act8(out, shape, "out", here))
     return out
 
 
@@ -318,11 +326,23 @@ def act8_unpack(a, out=None, dtype=torch.float32):
     """The values of a checkpoint as a float32 or bf16 tensor (both hold them exactly)."""
     if out is None:
         out = torch.empty(a.shape, dtype=dtype, device=a.codes.device)
-    _require_here(out, a.codes)
-    ld = _rows(out, "out", a.shape)
-    _emit("act8_unpack", a.desc, C.c_int64(a.shape[0]), C.c_int32(a.cols), _ptr(out), C.c_int32(_act_dtype(out, "out")),
-          C.c_int64(ld))
+    here = _device_of(out)
+    ld = _rows(out, "out", here, a.shape)
+    _emit("act8_unpack", _act8(a, a.shape, "the checkpoint", here), C.c_int64(a.shape[0]), C.c_int32(a.cols),
+          C.c_void_p(out.data_ptr()), C.c_int32(_act_dtype(out, "out")), C.c_int64(ld))
     return out
+
+
+def _workspace(workspace, need, like, here):
+    """(tensor, address, bytes) of a caller's scratch, or of a new one where it is too small."""
+    if workspace is not None:
+        have = workspace.numel()
+        if workspace.get_device() != here:
+            _elsewhere(workspace)
+        if have >= need:
+            return workspace, workspace.data_ptr(), have
+    workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    return workspace, workspace.data_ptr(), need
 
 
 # ------------------------------------------------------------- layer norm
@@ -335,20 +355,21 @@ def layer_norm_forward(x, gamma=None, beta=None, eps=1e-5, relu=False, out=None,
     xh = (x - mean) rstd.  Returns (y, mean, rstd); want_stats=False computes the statistics only where a buffer is given.
     xhat8 / y8: Act8 checkpoints of xh and of y that are written in the same pass for layer_norm_backward and for the next
     layer's backward pass.  y_absmax: see linear_forward.  out may be x."""
-    _require_here(x, gamma, beta, out, mean, rstd, y_absmax, _codes(xhat8), _codes(y8))
-    x_ld = _rows(x, "x")
+    here = _device_of(x)
+    x_ld = _rows(x, "x", here)
     M, N = shape = x.shape
+    dtype = x.dtype
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.dtype is not x.dtype:
-        raise TypeError("out must be %s like x, got %s" % (x.dtype, out.dtype))
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    elif out.dtype is not dtype:
+        raise TypeError("out must be %s like x, got %s" % (dtype, out.dtype))
     if want_stats:
         mean = torch.empty(M, dtype=torch.float32, device=x.device) if mean is None else mean
         rstd = torch.empty(M, dtype=torch.float32, device=x.device) if rstd is None else rstd
     _emit("layer_norm_forward", _capi.LayerNormDesc(
-        M, N, _act_dtype(x, "x"), x.data_ptr(), x_ld, _vector(gamma, N, "gamma"), _vector(beta, N, "beta"),
-        out.data_ptr(), _rows(out, "out", shape), _vector(mean, M, "mean"), _vector(rstd, M, "rstd"),
-        _act8(xhat8, shape, "xhat8"), _act8(y8, shape, "y8"), _vector(y_absmax, 1, "y_absmax"), eps,
+        M, N, _act_dtype(x, "x"), x.data_ptr(), x_ld, _vector(gamma, N, "gamma", here), _vector(beta, N, "beta", here),
+        out.data_ptr(), _rows(out, "out", here, shape), _vector(mean, M, "mean", here), _vector(rstd, M, "rstd", here),
+        _act8(xhat8, shape, "xhat8", here), _act8(y8, shape, "y8", here), _vector(y_absmax, 1, "y_absmax", here), eps,
         _capi.ACT_RELU if relu else _capi.ACT_NONE))
     return out, mean, rstd
 
@@ -366,10 +387,10 @@ def layer_norm_backward(dy, x, rstd, mean=None, gamma=None, relu_mask=None, out=
     """Backward pass of layer_norm_forward.  x: its input (with mean) or the Act8 of the normalised rows; relu_mask: its output
     or that output's Act8 where it had relu=True, else None.  Returns (dx, dgamma, dbeta, workspace); want_params=False
     computes the parameters' gradients only where a buffer is given.  out may be dy."""
-    _require_here(dy, rstd, mean, gamma, out, dgamma, dbeta, workspace, dx_absmax, _codes(x), _codes(relu_mask))
-    dy_ld = _rows(dy, "dy")
+    here = _device_of(dy)
+    dy_ld = _rows(dy, "dy", here)
     M, N = shape = dy.shape
-    dtype = _act_dtype(dy, "dy")
+    dtype = dy.dtype
     x_at = x_ld = mask_at = mask_ld = 0
     x8 = mask8 = None
     if isinstance(x, Act8):
@@ -377,34 +398,33 @@ def layer_norm_backward(dy, x, rstd, mean=None, gamma=None, relu_mask=None, out=
             raise ValueError("the checkpoint holds normalised rows: mean has no use")
         x8 = x
     else:
-        if x.dtype is not dy.dtype:
-            raise TypeError("x must be %s like dy, got %s" % (dy.dtype, x.dtype))
+        if x.dtype is not dtype:
+            raise TypeError("x must be %s like dy, got %s" % (dtype, x.dtype))
         if mean is None:
             raise ValueError("x needs the rows' means")
-        x_at, x_ld = x.data_ptr(), _rows(x, "x", shape)
+        x_at, x_ld = x.data_ptr(), _rows(x, "x", here, shape)
     if isinstance(relu_mask, Act8):
         mask8 = relu_mask
     elif relu_mask is not None:
-        if relu_mask.dtype is not dy.dtype:
-            raise TypeError("relu_mask must be %s like dy, got %s" % (dy.dtype, relu_mask.dtype))
-        mask_at, mask_ld = relu_mask.data_ptr(), _rows(relu_mask, "relu_mask", shape)
+        if relu_mask.dtype is not dtype:
+            raise TypeError("relu_mask must be %s like dy, got %s" % (dtype, relu_mask.dtype))
+        mask_at, mask_ld = relu_mask.data_ptr(), _rows(relu_mask, "relu_mask", here, shape)
     if out is None:
-        out = torch.empty(shape, dtype=dy.dtype, device=dy.device)
-    elif out.dtype is not dy.dtype:
-        raise TypeError("out must be %s like dy, got %s" % (dy.dtype, out.dtype))
+        out = torch.empty(shape, dtype=dtype, device=dy.device)
+    elif out.dtype is not dtype:
+        raise TypeError("out must be %s like dy, got %s" % (dtype, out.dtype))
     if want_params:
         dgamma = torch.empty(N, dtype=torch.float32, device=dy.device) if dgamma is None else dgamma
         dbeta = torch.empty(N, dtype=torch.float32, device=dy.device) if dbeta is None else dbeta
+    ws_at = ws_bytes = 0
     if dgamma is not None or dbeta is not None:
-        need = layer_norm_backward_workspace_bytes(M, N)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dy.device)
+        workspace, ws_at, ws_bytes = _workspace(workspace, layer_norm_backward_workspace_bytes(M, N), dy, here)
     _emit("layer_norm_backward", _capi.LayerNormBwdDesc(
-        M, N, dtype, x_at, x_ld, _act8(x8, shape, "x"), _vector(mean, M, "mean"), _vector(rstd, M, "rstd"),
-        _vector(gamma, N, "gamma"), dy.data_ptr(), dy_ld, mask_at, mask_ld, _act8(mask8, shape, "relu_mask"),
-        out.data_ptr(), _rows(out, "out", shape), _vector(dgamma, N, "dgamma"), _vector(dbeta, N, "dbeta"),
-        _vector(dx_absmax, 1, "dx_absmax")),
-        _ptr(workspace), C.c_size_t(0 if workspace is None else workspace.numel()))
+        M, N, _act_dtype(dy, "dy"), x_at, x_ld, _act8(x8, shape, "x", here), _vector(mean, M, "mean", here),
+        _vector(rstd, M, "rstd", here), _vector(gamma, N, "gamma", here), dy.data_ptr(), dy_ld, mask_at, mask_ld,
+        _act8(mask8, shape, "relu_mask", here), out.data_ptr(), _rows(out, "out", here, shape),
+        _vector(dgamma, N, "dgamma", here), _vector(dbeta, N, "dbeta", here), _vector(dx_absmax, 1, "dx_absmax", here)),
+        C.c_void_p(ws_at), C.c_size_t(ws_bytes))
     return out, dgamma, dbeta, workspace
 
 
@@ -412,8 +432,9 @@ def layer_norm_backward(dy, x, rstd, mean=None, gamma=None, relu_mask=None, out=
 
 
 def _ld(t):
-    assert t.dim() == 2 and t.stride(1) == 1, "need a row-major 2-D view"
-    return t.stride(0)
+    st = t.stride()
+    assert len(st) == 2 and st[1] == 1, "need a row-major 2-D view"
+    return st[0]
 
 
 class SplitWeights:
@@ -476,7 +497,6 @@ def linear_backward_data(dz, w, relu_mask=None, out=None, dz_absmax=None, w_absm
     mask8 = relu_mask if isinstance(relu_mask, Act8) else None
     if mask8 is not None:
         relu_mask = None
-        _require_here(dz, mask8.codes)
     _require_cuda(dz, w, relu_mask, out)
     M, N = dz.shape
     K = w.shape[1]
@@ -490,7 +510,7 @@ def linear_backward_data(dz, w, relu_mask=None, out=None, dz_absmax=None, w_absm
     if relu_mask is not None:
         d.d_relu_mask, d.relu_mask_ld = relu_mask.data_ptr(), _ld(relu_mask)
     elif mask8 is not None:
-        d.relu_mask8 = _act8(mask8, (M, K), "relu_mask")
+        d.relu_mask8 = _act8(mask8, (M, K), "relu_mask", _device_of(dz))
     d.gemm_mode = _gemm_field()
     d.d_dz_absmax, d.d_w_absmax, d.d_dx_absmax = _ptr0(dz_absmax), _ptr0(w_absmax), _ptr0(dx_absmax)
     if w_planes is not None:
@@ -526,9 +546,7 @@ def linear_backward_weight_workspace_bytes(M, N, K, act8=False):
 def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True, dz_absmax=None, x_absmax=None):
     """dW = dz^T x [N,K], db = column sums of dz.  x may be the Act8 of the activation.  *_absmax: see linear_forward."""
     x8 = x if isinstance(x, Act8) else None
-    if x8 is not None:
-        _require_here(dz, x8.codes)
-    _require_cuda(dz, _codes(x), dw, db, workspace)
+    _require_cuda(dz, x if x8 is None else None, dw, db, workspace)
     M, N = dz.shape
     K = x.shape[1]
     if dw is None:
@@ -542,7 +560,7 @@ def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True
     d.M, d.N, d.K = M, N, K
     d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
     if x8 is not None:
-        d.x8 = _act8(x8, (M, K), "x")
+        d.x8 = _act8(x8, (M, K), "x", _device_of(dz))
     else:
         d.d_x, d.x_ld = x.data_ptr(), _ld(x)
     d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)
@@ -557,16 +575,14 @@ def linear_backward_weight_static(dz, x, dw, db=None):
     """linear_backward_weight through the entry point that allocates nothing: partial sums go to the library's
     static device array (layers beyond its size are refused); outputs must be given."""
     x8 = x if isinstance(x, Act8) else None
-    if x8 is not None:
-        _require_here(dz, x8.codes)
-    _require_cuda(dz, _codes(x), dw, db)
+    _require_cuda(dz, x if x8 is None else None, dw, db)
     M, N = dz.shape
     K = x.shape[1]
     d = _capi.LinearBwdDesc()
     d.M, d.N, d.K = M, N, K
     d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
     if x8 is not None:
-        d.x8 = _act8(x8, (M, K), "x")
+        d.x8 = _act8(x8, (M, K), "x", _device_of(dz))
     else:
         d.d_x, d.x_ld = x.data_ptr(), _ld(x)
     d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)

@@ -270,8 +270,8 @@ int dlrm_split_weights(const dlrm_weight_planes *items, int32_t n, dlrm_stream_t
  * row-major (torch layout).  Any shape and leading dimension is accepted (K = 13, 479, ...);
  * operands whose rows start on 16-byte boundaries (pointer 16-byte aligned, leading dimension
  * a multiple of 4 floats) are read with 16-byte loads; others too, but for the operand's last row and a partial last
- * reduction step, which take 4-byte loads (DLRM_GEMM_F32_MFMA: 4-byte loads throughout).  Of rows on other boundaries
- * nothing past the view is read.  A leading dimension is a
+ * reduction step, which take 4-byte loads (DLRM_GEMM_F32_MFMA: 4-byte loads throughout).  Of an operand on other
+ * boundaries nothing behind the last row's last element is read.  A leading dimension is a
  * promise that every row, the last one included, is readable up to it: when x_ld and w_ld both reach K rounded
  * up to 32, the columns between K and that bound are loaded too (and discarded; they need not be zero).
  * Layers with at most 16 inputs or a single output are no matrix product and run in one-pass float32 fma kernels.
