@@ -53,6 +53,9 @@ class DLRMConfig:
     lr: float = 0.01
     eps: float = 1e-8
     name: str = "custom"
+    norm: bool = False            # hidden MLP layers are Linear + layer norm + ReLU (the reference: Linear + ReLU)
+    norm_eps: float = 1e-5
+    keep8: bool = False           # hidden activations wait for the backward pass as 8-bit checkpoints (ops.Act8)
 
     @staticmethod
     def mlperf(**kw):
@@ -115,26 +118,39 @@ def _padk(n):
 class MLPStack:
     """A stack of Linear+ReLU layers (struct Net2's fc1..fc4, src/dlrmtest.cpp:234-272).
     Weights [N, pad4(K)] and biases live in one flat parameter buffer shared by
-    all stacks of a model; gradients in its twin."""
+    all stacks of a model; gradients in its twin.
 
-    def __init__(self, sizes, params, grads, offset, last_relu=True):
+    norm: every layer but the last is Linear + layer norm + ReLU; gamma and beta follow the layer's bias.
+    keep8: what the backward pass needs of those layers waits for it in 8 bits (ops.Act8): the output, which is the next
+    layer's input and the ReLU's mask, and with norm the normalised rows.  Their float32 outputs then share two buffers
+    (hidden_buffers): a layer's is only read by the layer after it."""
+
+    def __init__(self, sizes, params, grads, offset, last_relu=True, norm=False, norm_eps=1e-5, keep8=False):
         self.sizes = list(sizes)
         self.last_relu = last_relu
+        self.norm, self.norm_eps, self.keep8 = norm, norm_eps, keep8
         self.W, self.b, self.dW, self.db = [], [], [], []
+        self.gamma, self.beta, self.dgamma, self.dbeta = [], [], [], []
         o = offset
-        for K, N in zip(sizes[:-1], sizes[1:]):
+        for i, (K, N) in enumerate(zip(sizes[:-1], sizes[1:])):
             kp = _padk(K)
             self.W.append(params[o:o + N * kp].view(N, kp)[:, :K])
             self.dW.append(grads[o:o + N * kp].view(N, kp)[:, :K])
             o += N * kp
-            self.b.append(params[o:o + N])
-            self.db.append(grads[o:o + N])
-            o += _pad4(N)
+            vectors = [(self.b, self.db)]
+            if norm and i + 2 < len(sizes):
+                vectors += [(self.gamma, self.dgamma), (self.beta, self.dbeta)]
+            for v, dv in vectors:
+                v.append(params[o:o + N])
+                dv.append(grads[o:o + N])
+                o += _pad4(N)
         self.end = o
+        self.ws_norm = None
 
     @staticmethod
-    def param_count(sizes):
-        return sum(N * _padk(K) + _pad4(N) for K, N in zip(sizes[:-1], sizes[1:]))
+    def param_count(sizes, norm=False):
+        hidden = sum(2 * _pad4(N) for N in sizes[1:-1]) if norm else 0
+        return hidden + sum(N * _padk(K) + _pad4(N) for K, N in zip(sizes[:-1], sizes[1:]))
 
     @property
     def n_layers(self):
@@ -148,14 +164,62 @@ class MLPStack:
             N, K = W.shape
             W.copy_((torch.randn(N, K, generator=gen) * (2.0 / (K + N)) ** 0.5).to(W.device))
             b.copy_((torch.randn(N, generator=gen) * (1.0 / N) ** 0.5).to(b.device))
+        for g, e in zip(self.gamma, self.beta):
+            g.fill_(1.0)
+            e.zero_()
 
-    def forward(self, x, acts):
-        """acts[i] receives the output of layer i ([B, N_i] views)."""
+    def hidden_buffers(self, batch, device):
+        """The float32 outputs of the hidden layers ([B, N_i] views), and what the backward pass keeps of them."""
+        widths = self.sizes[1:-1]
+        f32 = dict(dtype=torch.float32, device=device)
+        if self.keep8:
+            pair = [torch.zeros(batch * max([_padk(n) for n in widths[k::2]] or [0]), **f32) for k in (0, 1)]
+            acts = [pair[i % 2][:batch * _padk(n)].view(batch, _padk(n))[:, :n] for i, n in enumerate(widths)]
+            self.y8 = [ops.Act8.empty(batch, n, device) for n in widths]
+            self.xhat8 = [ops.Act8.empty(batch, n, device) for n in widths] if self.norm else []
+        else:
+            acts = [torch.zeros((batch, _padk(n)), **f32)[:, :n] for n in widths]
+            self.z = [torch.zeros((batch, _padk(n)), **f32)[:, :n] for n in widths] if self.norm else []
+            self.mean = [torch.zeros(batch, **f32) for _ in widths] if self.norm else []
+        self.rstd = [torch.zeros(batch, **f32) for _ in widths] if self.norm else []
+        return acts
+
+    def forward(self, x, acts, keep=True):
+        """acts[i] receives the output of layer i ([B, N_i] views).  keep=False: no backward pass follows (nothing is kept
+        in 8 bits)."""
+        keep = keep and self.keep8
         for i in range(self.n_layers):
-            relu = self.last_relu or i + 1 < self.n_layers
-            ops.linear_forward(x, self.W[i], self.b[i], relu, out=acts[i])
+            hidden = i + 1 < self.n_layers
+            if hidden and self.norm:
+                z = acts[i] if self.keep8 else self.z[i]
+                ops.linear_forward(x, self.W[i], self.b[i], False, out=z)
+                ops.layer_norm_forward(z, self.gamma[i], self.beta[i], eps=self.norm_eps, relu=True, out=acts[i],
+                                       mean=None if self.keep8 else self.mean[i], rstd=self.rstd[i], want_stats=False,
+                                       xhat8=self.xhat8[i] if keep else None, y8=self.y8[i] if keep else None)
+            else:
+                ops.linear_forward(x, self.W[i], self.b[i], self.last_relu or hidden, out=acts[i])
+                if hidden and keep:
+                    ops.act8_pack(acts[i], out=self.y8[i])
             x = acts[i]
         return x
+
+    def kept(self, i, x_in, acts):
+        """What the backward pass reads for the input of layer i."""
+        if i == 0:
+            return x_in
+        return self.y8[i - 1] if self.keep8 else acts[i - 1]
+
+    def input_gradient(self, i, dz, acts, out):
+        """Gradient of layer i's input, i > 0, carried through the ReLU (and the norm) in front of it: layer i-1's dz."""
+        if not self.norm:
+            return ops.linear_backward_data(dz, self.W[i], relu_mask=self.kept(i, None, acts), out=out)
+        ops.linear_backward_data(dz, self.W[i], out=out)
+        h = i - 1
+        _, _, _, self.ws_norm = ops.layer_norm_backward(
+            out, self.xhat8[h] if self.keep8 else self.z[h], self.rstd[h], mean=None if self.keep8 else self.mean[h],
+            gamma=self.gamma[h], relu_mask=self.kept(i, None, acts), out=out, dgamma=self.dgamma[h], dbeta=self.dbeta[h],
+            workspace=self.ws_norm)
+        return out
 
     def backward(self, x_in, acts, dz_last, dz_bufs, ws, dx_first=None):
         """dz_last: gradient w.r.t. the last layer's pre-activation.  dz_bufs[i]
@@ -163,10 +227,9 @@ class MLPStack:
         i < last.  If dx_first is given it receives d(loss)/d(x_in), unmasked."""
         dz = dz_last
         for i in reversed(range(self.n_layers)):
-            x = x_in if i == 0 else acts[i - 1]
-            _, _, ws = ops.linear_backward_weight(dz, x, dw=self.dW[i], db=self.db[i], workspace=ws)
+            _, _, ws = ops.linear_backward_weight(dz, self.kept(i, x_in, acts), dw=self.dW[i], db=self.db[i], workspace=ws)
             if i > 0:
-                dz = ops.linear_backward_data(dz, self.W[i], relu_mask=acts[i - 1], out=dz_bufs[i - 1])
+                dz = self.input_gradient(i, dz, acts, dz_bufs[i - 1])
             elif dx_first is not None:
                 ops.linear_backward_data(dz, self.W[0], out=dx_first)
         return ws
@@ -289,11 +352,12 @@ class DLRM:
         # ---- dense parameters: one flat buffer (+ twin for gradients)
         bsz = [cfg.dense_in] + list(cfg.bottom)
         tsz = [cfg.top_in] + list(cfg.top)
-        n_par = MLPStack.param_count(bsz) + MLPStack.param_count(tsz)
+        n_par = MLPStack.param_count(bsz, cfg.norm) + MLPStack.param_count(tsz, cfg.norm)
         self.params = torch.zeros(n_par, dtype=torch.float32, device=dev)
         self.grads = torch.zeros(n_par, dtype=torch.float32, device=dev)
-        self.bottom = MLPStack(bsz, self.params, self.grads, 0, last_relu=True)
-        self.top = MLPStack(tsz, self.params, self.grads, self.bottom.end, last_relu=cfg.final_relu)
+        hidden = dict(norm=cfg.norm, norm_eps=cfg.norm_eps, keep8=cfg.keep8)
+        self.bottom = MLPStack(bsz, self.params, self.grads, 0, last_relu=True, **hidden)
+        self.top = MLPStack(tsz, self.params, self.grads, self.bottom.end, last_relu=cfg.final_relu, **hidden)
         gen = torch.Generator().manual_seed(seed)  # same on every rank: replicas start identical
         self.bottom.init_(gen)
         self.top.init_(gen)
@@ -316,10 +380,10 @@ class DLRM:
             self.feat = torch.zeros((B, self.inter_ld), **f32)    # [bottom out | pooled tables], read by the top MLP
             self.dfeat = torch.zeros((B, self.inter_ld), **f32)
             self.inter, self.dinter = self.feat, self.dfeat
-        self.bot_acts = [torch.zeros((B, _padk(n)), **f32)[:, :n] for n in cfg.bottom[:-1]]
+        self.bot_acts = self.bottom.hidden_buffers(B, dev)
         self.bot_acts.append(self.feat[:, :cfg.bottom[-1]])
         self.bot_dz = [torch.zeros((B, _padk(n)), **f32)[:, :n] for n in cfg.bottom[:-1]]
-        self.top_acts = [torch.zeros((B, _padk(n)), **f32)[:, :n] for n in cfg.top[:-1]]
+        self.top_acts = self.top.hidden_buffers(B, dev)
         self.pred = torch.zeros((B, 1), **f32)
         self.top_acts.append(self.pred)
         self.top_dz = [torch.zeros((B, _padk(n)), **f32)[:, :n] for n in cfg.top[:-1]]
@@ -619,14 +683,14 @@ class DLRM:
         items = self._presort_items(indices, offsets) if train else []
         items.append(("wait", "emb", "main"))    # earlier readers of feat and the input copies are done
         items += self._emb_forward_items(indices, offsets)
-        items.append(("ops", "main", lambda: self.bottom.forward(self.x_dense[:, :cfg.dense_in], self.bot_acts)))
+        items.append(("ops", "main", lambda: self.bottom.forward(self.x_dense[:, :cfg.dense_in], self.bot_acts, keep=train)))
         items.append(("wait", "main", "emb"))
 
         def top():
             if cfg.interaction == "dot":
                 ops.interact_dot_forward(self.feat.view(self.B, cfg.num_features, cfg.dim), out=self.inter,
                                          out_ld=self.inter_ld)
-            self.top.forward(self.inter[:, :cfg.top_in], self.top_acts)
+            self.top.forward(self.inter[:, :cfg.top_in], self.top_acts, keep=train)
         items.append(("ops", "main", top))
         return items
 
@@ -640,7 +704,7 @@ class DLRM:
         items = []
         for i in reversed(range(stack.n_layers)):
             dz = dz_last if i == stack.n_layers - 1 else dz_bufs[i]
-            x = x_in if i == 0 else acts[i - 1]
+            x = stack.kept(i, x_in, acts)
 
             def wgrad(dz=dz, x=x, i=i):
                 _, _, self.ws_dense = ops.linear_backward_weight(dz, x, dw=stack.dW[i], db=stack.db[i],
@@ -648,8 +712,7 @@ class DLRM:
             items.append(("wait", "wgrad", "main"))          # dz of this layer is complete
             items.append(("ops", "wgrad", wgrad))
             if i > 0:
-                items.append(("ops", "main", lambda dz=dz, i=i: ops.linear_backward_data(
-                    dz, stack.W[i], relu_mask=acts[i - 1], out=dz_bufs[i - 1])))
+                items.append(("ops", "main", lambda dz=dz, i=i: stack.input_gradient(i, dz, acts, dz_bufs[i - 1])))
             elif dx_first is not None:
                 items.append(("ops", "main", lambda dz=dz: ops.linear_backward_data(dz, stack.W[0], out=dx_first)))
         return items
