@@ -10,6 +10,7 @@ namespace dlrm {
 
 int act8_check(const dlrm_act8 *a, int cols, const char *what) {
     DLRM_REQUIRE(a->d_codes != nullptr && a->d_exps != nullptr, "%s: NULL codes or exponents", what);
+    DLRM_REQUIRE(cols <= (1 << 30), "%s: %d columns are more than 2^30", what, cols);
     const int64_t blocks = act8_blocks(cols);
     DLRM_REQUIRE(reinterpret_cast<uintptr_t>(a->d_codes) % 16 == 0 && a->ld % 16 == 0,
                  "%s: code rows must start on 16-byte boundaries (leading dimension %lld)", what, (long long)a->ld);

@@ -32,6 +32,15 @@ struct dlrm_plan {
         }                                                        \
     } while (0)
 
+// no exception leaves a C entry: what std::function or the vector throws becomes -1 with a message
+#define PLAN_TRY(expr)                                                       \
+    try {                                                                    \
+        return expr;                                                         \
+    } catch (...) {                                                          \
+        ::dlrm::set_error(DLRM_ERR_NOMEM, "no memory for another entry");    \
+        return -1;                                                           \
+    }
+
 namespace {
 
 int idx_size(int32_t idx_dtype) { return idx_dtype == DLRM_I64 ? 8 : 4; }
@@ -207,31 +216,31 @@ extern "C" int dlrm_plan_add_act8_pack(dlrm_plan *p, const void *d_x, int32_t dt
                                        const dlrm_act8 *out) {
     PLAN_REQUIRE(p != nullptr && out != nullptr, "bad arguments");
     const dlrm_act8 a = *out;
-    return add(p, DLRM_OP_ACT8_PACK,
-               [=](dlrm_plan *, hipStream_t s) { return dlrm_act8_pack(d_x, dtype, rows, cols, x_ld, &a, s); });
+    PLAN_TRY(add(p, DLRM_OP_ACT8_PACK,
+                 [=](dlrm_plan *, hipStream_t s) { return dlrm_act8_pack(d_x, dtype, rows, cols, x_ld, &a, s); }))
 }
 
 extern "C" int dlrm_plan_add_act8_unpack(dlrm_plan *p, const dlrm_act8 *a, int64_t rows, int32_t cols, void *d_x, int32_t dtype,
                                          int64_t x_ld) {
     PLAN_REQUIRE(p != nullptr && a != nullptr, "bad arguments");
     const dlrm_act8 d = *a;
-    return add(p, DLRM_OP_ACT8_UNPACK,
-               [=](dlrm_plan *, hipStream_t s) { return dlrm_act8_unpack(&d, rows, cols, d_x, dtype, x_ld, s); });
+    PLAN_TRY(add(p, DLRM_OP_ACT8_UNPACK,
+                 [=](dlrm_plan *, hipStream_t s) { return dlrm_act8_unpack(&d, rows, cols, d_x, dtype, x_ld, s); }))
 }
 
 extern "C" int dlrm_plan_add_layer_norm_forward(dlrm_plan *p, const dlrm_layer_norm *l) {
     PLAN_REQUIRE(p != nullptr && l != nullptr, "bad arguments");
     const dlrm_layer_norm d = *l;
-    return add(p, DLRM_OP_LAYER_NORM_FORWARD, [d](dlrm_plan *, hipStream_t s) { return dlrm_layer_norm_forward(&d, s); });
+    PLAN_TRY(add(p, DLRM_OP_LAYER_NORM_FORWARD, [d](dlrm_plan *, hipStream_t s) { return dlrm_layer_norm_forward(&d, s); }))
 }
 
 extern "C" int dlrm_plan_add_layer_norm_backward(dlrm_plan *p, const dlrm_layer_norm_bwd *l, void *d_workspace,
                                                  size_t workspace_bytes) {
     PLAN_REQUIRE(p != nullptr && l != nullptr, "bad arguments");
     const dlrm_layer_norm_bwd d = *l;
-    return add(p, DLRM_OP_LAYER_NORM_BACKWARD, [d, d_workspace, workspace_bytes](dlrm_plan *, hipStream_t s) {
+    PLAN_TRY(add(p, DLRM_OP_LAYER_NORM_BACKWARD, [d, d_workspace, workspace_bytes](dlrm_plan *, hipStream_t s) {
         return dlrm_layer_norm_backward(&d, d_workspace, workspace_bytes, s);
-    });
+    }))
 }
 
 extern "C" int dlrm_plan_enable_timing(dlrm_plan *p, int32_t max_runs) {

@@ -325,6 +325,7 @@ int dlrm_absmax(const float *d_x, int64_t rows, int32_t cols, int64_t ld, float 
  *                    They are exact bf16 numbers, so dz alone is cut into its
  *                    three bf16 pieces and the product has float32 accuracy
  *                    from three bf16 terms; gemm_mode has no say in it.
+ *                    Leading dimensions of dz and x8 up to 2^24.
  */
 typedef struct dlrm_linear_bwd {
     int64_t M;

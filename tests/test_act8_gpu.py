@@ -213,3 +213,23 @@ def test_checkpoint_of_another_shape_is_refused():
         ops.act8_pack(torch.ones((8, 40), device="cuda", dtype=torch.float16))
     with pytest.raises(ValueError):
         ops.act8_pack(torch.ones((40, 8), device="cuda").t())
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 codes: the last rows are what a call on them alone gives.  Small whole numbers, so every sum is exact."""
+    from dlrm_amd import ops
+    M, K, N, tail = (1 << 22) + 77, 1024, 4, 300
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+    x[-tail:] = torch.randint(-8, 9, (tail, K), device="cuda").to(torch.bfloat16)
+    a = ops.act8_pack(x)
+    last = ops.act8_pack(x[-tail:])
+    assert torch.equal(a.codes[-tail:], last.codes) and torch.equal(a.exps[-tail:], last.exps)
+    assert not a.codes[:tail].any()
+    back = ops.act8_unpack(a, dtype=torch.bfloat16)
+    assert torch.equal(back[-tail:], x[-tail:]) and not back[:tail].any()
+    del back
+    dz = torch.zeros((M, N), device="cuda")
+    dz[-tail:] = torch.randint(-3, 4, (tail, N), device="cuda").float()
+    dw, db, _ = ops.linear_backward_weight(dz, a)
+    want, want_b, _ = ops.linear_backward_weight(dz[-tail:], last)
+    assert want.any() and torch.equal(dw, want) and torch.equal(db, want_b)

@@ -122,6 +122,10 @@ def test_linear_backward_refuses_mixed_operands():
     d.d_x = 0
     d.x8 = act8(ld=32)
     refused(L.dlrm_linear_backward_weight(C.byref(d), C.c_void_p(P), C.c_size_t(1 << 30), None), "too small")
+    d.x8, d.K, d.dw_ld = act8(ld=1 << 31, exps_ld=1 << 26), (1 << 30) + 1, 1 << 31
+    refused(L.dlrm_linear_backward_weight(C.byref(d), C.c_void_p(P), C.c_size_t(1 << 62), None), "2^30")
+    d.x8, d.K, d.dw_ld = act8(ld=(1 << 24) + 16), 40, 40
+    refused(L.dlrm_linear_backward_weight(C.byref(d), C.c_void_p(P), C.c_size_t(1 << 30), None), "2^24")
     d.x8 = act8(codes=0)
     refused(L.dlrm_linear_backward_weight(C.byref(d), C.c_void_p(P), C.c_size_t(1 << 30), None), "NULL")
     d.d_relu_mask, d.relu_mask_ld, d.relu_mask8 = P, 40, act8()

@@ -387,3 +387,27 @@ def test_normalised_layers_train_from_checkpoints():
     assert float((out.cpu().double() - y).abs().max()) <= 1e-5 * float(y.abs().max())
     for n in ref:
         assert float((grads[n].cpu().double() - ref[n]).abs().max()) <= 1e-5 * float(ref[n].abs().max()), n
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements, and rows 2^31 elements apart: the last rows are what a call on them alone gives."""
+    from dlrm_amd import ops
+    M, N, tail = (1 << 22) + 77, 1024, 300
+    x = torch.zeros((M, N), dtype=torch.bfloat16, device="cuda")
+    x[-tail:] = torch.randn(tail, N, device="cuda").to(torch.bfloat16)
+    xhat8 = ops.Act8.empty(M, N)
+    y, mean, rstd = ops.layer_norm_forward(x, relu=True, xhat8=xhat8)
+    a8 = ops.Act8.empty(tail, N)
+    ya, ma, ra = ops.layer_norm_forward(x[-tail:], relu=True, xhat8=a8)
+    assert torch.equal(y[-tail:], ya) and torch.equal(mean[-tail:], ma) and torch.equal(rstd[-tail:], ra)
+    assert torch.equal(xhat8.codes[-tail:], a8.codes) and torch.equal(xhat8.exps[-tail:], a8.exps)
+    for source, short, m, s in ((x, x[-tail:], mean, ma), (xhat8, a8, None, None)):
+        dx, _, db, _ = ops.layer_norm_backward(x, source, rstd, mean=m, relu_mask=y, want_params=False)
+        dxa, _, _, _ = ops.layer_norm_backward(x[-tail:], short, ra, mean=s, relu_mask=ya, want_params=False)
+        assert torch.equal(dx[-tail:], dxa) and not dx[:tail].any()
+        del dx
+    del y, xhat8
+    apart = x.view(-1).as_strided((2, 64), ((1 << 31) + 8, 1))
+    apart.copy_(torch.randn(2, 64, device="cuda"))
+    near = apart.clone()
+    assert torch.equal(ops.layer_norm_forward(apart, out=apart)[0], ops.layer_norm_forward(near)[0])
