@@ -100,9 +100,9 @@ class LayerNormDesc(C.Structure):
         ("d_gamma", C.c_void_p), ("d_beta", C.c_void_p),
         ("d_y", C.c_void_p), ("y_ld", C.c_int64),
         ("d_mean", C.c_void_p), ("d_rstd", C.c_void_p),
-        ("xhat8", Act8Desc), ("y8", Act8Desc),
         ("d_y_absmax", C.c_void_p),
         ("eps", C.c_float), ("act", C.c_int32),
+        ("xhat8", Act8Desc), ("y8", Act8Desc),
     ]
 
 
@@ -110,14 +110,13 @@ class LayerNormBwdDesc(C.Structure):
     _fields_ = [
         ("M", C.c_int64), ("N", C.c_int32), ("dtype", C.c_int32),
         ("d_x", C.c_void_p), ("x_ld", C.c_int64),
-        ("xhat8", Act8Desc),
         ("d_mean", C.c_void_p), ("d_rstd", C.c_void_p), ("d_gamma", C.c_void_p),
         ("d_dy", C.c_void_p), ("dy_ld", C.c_int64),
         ("d_relu_mask", C.c_void_p), ("relu_mask_ld", C.c_int64),
-        ("relu_mask8", Act8Desc),
         ("d_dx", C.c_void_p), ("dx_ld", C.c_int64),
         ("d_dgamma", C.c_void_p), ("d_dbeta", C.c_void_p),
         ("d_dx_absmax", C.c_void_p),
+        ("xhat8", Act8Desc), ("relu_mask8", Act8Desc),
     ]
 
 

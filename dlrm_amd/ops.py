@@ -268,15 +268,16 @@ class Act8:
     def __init__(self, codes, exps, cols):
         if codes.dtype is not torch.int8 or exps.dtype is not torch.uint8:
             raise TypeError("codes must be int8 and exponents uint8, got %s and %s" % (codes.dtype, exps.dtype))
-        blocks = (cols + 31) // 32
-        here = codes.get_device()
-        ld, exps_ld = _rows(codes, "codes", here), _rows(exps, "exponents", exps.get_device())
-        (rows, width), (exp_rows, exp_width) = codes.shape, exps.shape
-        if cols < 1 or exp_rows != rows or width < 32 * blocks or exp_width < blocks:
-            raise ValueError("%d columns need codes [rows, %d] and exponents [rows, %d], got %s and %s"
-                             % (cols, 32 * blocks, blocks, tuple(codes.shape), tuple(exps.shape)))
+        blocks, here = (cols + 31) // 32, codes.get_device()
+        s, t, st, tt = codes.shape, exps.shape, codes.stride(), exps.stride()
+        if (cols < 1 or len(s) != 2 or len(t) != 2 or s[0] != t[0] or s[1] < 32 * blocks or t[1] < blocks or st[1] != 1
+                or (tt[1] != 1 and t[1] > 1)):
+            raise ValueError("%d columns need row-major codes [rows, %d] and exponents [rows, %d], got shapes %s and %s, strides "
+                             "%s and %s" % (cols, 32 * blocks, blocks, tuple(s), tuple(t), st, tt))
         if exps.get_device() != here:
             raise ValueError("codes and exponents live on different devices")
+        rows = s[0]
+        ld, exps_ld = (st[0], tt[0]) if rows > 1 else (max(st[0], s[1]), max(tt[0], t[1]))
         if rows == 1:
             ld = (ld + 15) // 16 * 16
         at = codes.data_ptr()
@@ -292,13 +293,8 @@ class Act8:
                     torch.empty((rows, blocks), dtype=torch.uint8, device=device), cols)
 
 
-_no_act8 = _capi.Act8Desc()
-
-
 def _act8(a, shape, what, here):
-    """Descriptor of a checkpoint on device `here` that must have this shape (None: an empty one)."""
-    if a is None:
-        return _no_act8
+    """Descriptor of a checkpoint on device `here` that must have this shape."""
     if not isinstance(a, Act8):
         raise TypeError("%s must be an Act8, got %s" % (what, type(a).__name__))
     if a.shape != shape:
@@ -366,11 +362,15 @@ def layer_norm_forward(x, gamma=None, beta=None, eps=1e-5, relu=False, out=None,
     if want_stats:
         mean = torch.empty(M, dtype=torch.float32, device=x.device) if mean is None else mean
         rstd = torch.empty(M, dtype=torch.float32, device=x.device) if rstd is None else rstd
-    _emit("layer_norm_forward", _capi.LayerNormDesc(
+    d = _capi.LayerNormDesc(
         M, N, _act_dtype(x, "x"), x.data_ptr(), x_ld, _vector(gamma, N, "gamma", here), _vector(beta, N, "beta", here),
         out.data_ptr(), _rows(out, "out", here, shape), _vector(mean, M, "mean", here), _vector(rstd, M, "rstd", here),
-        _act8(xhat8, shape, "xhat8", here), _act8(y8, shape, "y8", here), _vector(y_absmax, 1, "y_absmax", here), eps,
-        _capi.ACT_RELU if relu else _capi.ACT_NONE))
+        _vector(y_absmax, 1, "y_absmax", here), eps, _capi.ACT_RELU if relu else _capi.ACT_NONE)
+    if xhat8 is not None:
+        d.xhat8 = _act8(xhat8, shape, "xhat8", here)
+    if y8 is not None:
+        d.y8 = _act8(y8, shape, "y8", here)
+    _emit("layer_norm_forward", d)
     return out, mean, rstd
 
 
@@ -419,12 +419,15 @@ def layer_norm_backward(dy, x, rstd, mean=None, gamma=None, relu_mask=None, out=
     ws_at = ws_bytes = 0
     if dgamma is not None or dbeta is not None:
         workspace, ws_at, ws_bytes = _workspace(workspace, layer_norm_backward_workspace_bytes(M, N), dy, here)
-    _emit("layer_norm_backward", _capi.LayerNormBwdDesc(
-        M, N, _act_dtype(dy, "dy"), x_at, x_ld, _act8(x8, shape, "x", here), _vector(mean, M, "mean", here),
-        _vector(rstd, M, "rstd", here), _vector(gamma, N, "gamma", here), dy.data_ptr(), dy_ld, mask_at, mask_ld,
-        _act8(mask8, shape, "relu_mask", here), out.data_ptr(), _rows(out, "out", here, shape),
-        _vector(dgamma, N, "dgamma", here), _vector(dbeta, N, "dbeta", here), _vector(dx_absmax, 1, "dx_absmax", here)),
-        C.c_void_p(ws_at), C.c_size_t(ws_bytes))
+    d = _capi.LayerNormBwdDesc(
+        M, N, _act_dtype(dy, "dy"), x_at, x_ld, _vector(mean, M, "mean", here), _vector(rstd, M, "rstd", here),
+        _vector(gamma, N, "gamma", here), dy.data_ptr(), dy_ld, mask_at, mask_ld, out.data_ptr(), _rows(out, "out", here, shape),
+        _vector(dgamma, N, "dgamma", here), _vector(dbeta, N, "dbeta", here), _vector(dx_absmax, 1, "dx_absmax", here))
+    if x8 is not None:
+        d.xhat8 = _act8(x8, shape, "x", here)
+    if mask8 is not None:
+        d.relu_mask8 = _act8(mask8, shape, "relu_mask", here)
+    _emit("layer_norm_backward", d, C.c_void_p(ws_at), C.c_size_t(ws_bytes))
     return out, dgamma, dbeta, workspace
 
 

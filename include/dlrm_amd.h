@@ -410,11 +410,11 @@ typedef struct dlrm_layer_norm {
     int64_t y_ld;
     float *d_mean;         /* [M] or NULL */
     float *d_rstd;         /* [M] or NULL */
-    dlrm_act8 xhat8;       /* [M,N], d_codes NULL: not written */
-    dlrm_act8 y8;          /* [M,N], d_codes NULL: not written */
     float *d_y_absmax;     /* or NULL: max |y| is folded in with atomicMax (start it at 0; see dlrm_linear) */
     float eps;
     int32_t act;           /* DLRM_ACT_NONE | DLRM_ACT_RELU */
+    dlrm_act8 xhat8;       /* [M,N], d_codes NULL: not written */
+    dlrm_act8 y8;          /* [M,N], d_codes NULL: not written */
 } dlrm_layer_norm;
 
 int dlrm_layer_norm_forward(const dlrm_layer_norm *l, dlrm_stream_t stream);
@@ -434,7 +434,6 @@ typedef struct dlrm_layer_norm_bwd {
     int32_t dtype;             /* of x, y, dy and dx */
     const void *d_x;           /* [M,N] or NULL */
     int64_t x_ld;
-    dlrm_act8 xhat8;           /* [M,N] in place of d_x */
     const float *d_mean;       /* [M] (with d_x) */
     const float *d_rstd;       /* [M] */
     const float *d_gamma;      /* [N] or NULL (1) */
@@ -442,12 +441,13 @@ typedef struct dlrm_layer_norm_bwd {
     int64_t dy_ld;
     const void *d_relu_mask;   /* [M,N] or NULL */
     int64_t relu_mask_ld;
-    dlrm_act8 relu_mask8;      /* [M,N] in place of d_relu_mask */
     void *d_dx;                /* [M,N] */
     int64_t dx_ld;
     float *d_dgamma;           /* [N] or NULL */
     float *d_dbeta;            /* [N] or NULL */
     float *d_dx_absmax;        /* or NULL: max |dx| is folded in with atomicMax */
+    dlrm_act8 xhat8;           /* [M,N] in place of d_x */
+    dlrm_act8 relu_mask8;      /* [M,N] in place of d_relu_mask */
 } dlrm_layer_norm_bwd;
 
 int dlrm_layer_norm_backward_workspace_bytes(int64_t M, int32_t N, size_t *bytes);
