@@ -335,6 +335,8 @@ def _workspace(workspace, need, like, here):
         have = workspace.numel()
         if workspace.get_device() != here:
             _elsewhere(workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("the workspace must be contiguous")
         if have >= need:
             return workspace, workspace.data_ptr(), have
     workspace = torch.empty(need, dtype=torch.uint8, device=like.device)

@@ -135,6 +135,22 @@ def test_backward(M, N, kept, pad, dtype):
     assert (buf == 7.0).all()
 
 
+@pytest.mark.parametrize("M,N", [(1, 24), (33, 24), (5, 100), (1025, 256), (3, 300), (2, 1500), (1, 1500)])
+def test_in_place_with_maxima(M, N):
+    """The output over the input, in batches whose last rows do not fill a workgroup: its largest magnitude is that of the rows."""
+    from dlrm_amd import ops
+    x, gamma, beta, dy = (t.cuda() for t in inputs(M, N, torch.float32, seed=17))
+    y, mean, rstd = ops.layer_norm_forward(x, gamma * 1e-3, beta * 1e-3)
+    dx, _, _, _ = ops.layer_norm_backward(dy, x, rstd, mean=mean, gamma=gamma * 1e-3)
+    for _ in range(5):
+        top, into = torch.zeros(1, device="cuda"), x.clone()
+        ops.layer_norm_forward(into, gamma * 1e-3, beta * 1e-3, out=into, y_absmax=top)
+        assert torch.equal(into, y) and top.item() == y.abs().max().item()
+        top, into = torch.zeros(1, device="cuda"), dy.clone()
+        ops.layer_norm_backward(into, x, rstd, mean=mean, gamma=gamma * 1e-3, out=into, dx_absmax=top)
+        assert torch.equal(into, dx) and top.item() == dx.abs().max().item()
+
+
 def test_gradient_against_differences():
     """dx, dgamma and dbeta against central differences of the float64 forward formula, contracted with random directions: the
     differences of a loss L = sum(y r) with a step of 1e-5 are exact to about 1e-9 of the gradients' size, the kernel's own
@@ -236,6 +252,7 @@ def test_refusals_before_a_launch():
            lambda: ops.layer_norm_backward(x, x, s), lambda: ops.layer_norm_backward(x, a, s, mean=s),
            lambda: ops.layer_norm_backward(x, x.bfloat16(), s, mean=s), lambda: ops.layer_norm_backward(x, x[:3], s, mean=s),
            lambda: ops.layer_norm_backward(x, a, s, relu_mask=x[:, :39]), lambda: ops.layer_norm_backward(x, a, v),
+           lambda: ops.layer_norm_backward(x, a, s, workspace=torch.empty(1, dtype=torch.uint8, device="cuda").expand(1 << 20)),
            lambda: ops.layer_norm_backward(x, a, s, dgamma=s), lambda: ops.layer_norm_backward(x, ops.Act8.empty(4, 41), s)]
     from dlrm_amd._capi import DlrmError
     for call in bad:
