@@ -14,7 +14,7 @@
 // atomics, the same bits every time.
 //
 // Measured (a 1 GiB copy reaches 5.1 to 5.4 TB/s here): forward 65536 x 1024 float32 97 us = 5.5 TB/s, with both checkpoints
-// 138 us = 4.9; backward 202 us = 5.3 TB/s from x with a mask, 124 us = 5.4 from the checkpoints; bf16 63 us = 4.3 forward,
+// 138 us = 4.9; backward 202 us = 5.3 TB/s from x with a mask, 124 us = 5.4 from the checkpoints; bf16 56 us = 4.8 forward,
 // 104 us = 5.2 backward from x.  Rows of 16384 float32 from a checkpoint spill (213 us, 3.2 TB/s).
 #include "act8.h"
 
@@ -485,16 +485,22 @@ __global__ __launch_bounds__(1024) void param_sums_kernel(ParamSums p) {
 // ---- launches.  Rows per width: a team of 8 to 64 lanes with up to 32 elements a lane, then 256 and 1024 threads.
 // Most partial rows that a backward launch leaves, which are its workgroups: two per compute unit (us from x, float32:
 // 8192 x 512 14.0 with 512 workgroups, 15.6 with 256, 14.4 with 1024; 8192 x 1024 21.7, 24.3, 23.7).  Requesting the next
-// row ahead of a row's sums was measured at no gain (14.1, 21.9): other waves cover the wait.
-static int64_t norm_bwd_parts(int64_t M, int N) {
-    const int64_t cap = N <= 8192 ? 512 : (N <= kLongRow ? 256 : 64);
+// row ahead of a row's sums was measured at no gain (14.1, 21.9): other waves cover the wait.  bf16 rows up to 2048 have one
+// piece a lane in flight and take four per compute unit (65536 x 1024 from x 104 against 142 us, 8192 x 1024 20.2 against
+// 21.0; 2048: 117 us; 16384 x 4096 127 against 122 with two).
+static int64_t norm_bwd_cap(int N, bool bf16) { return N <= 2048 && bf16 ? 1024 : N <= 8192 ? 512 : (N <= kLongRow ? 256 : 64); }
+static int64_t norm_bwd_parts(int64_t M, int N, bool bf16 = true) {        // (a workspace holds either type's)
+    const int64_t cap = norm_bwd_cap(N, bf16);
     return M < cap ? (M < 1 ? 1 : M) : cap;
 }
 
+// Forward workgroups of 256 threads at most, each with several rows: 16 per compute unit where a lane has one or two pieces
+// (us, 2048 / 4096 / 8192 workgroups: bf16 65536 x 1024 66.6 / 56.2 / 56.7, 32768 x 512 16.6 / 16.2 / 18.2, float32
+// 262144 x 256 120 / 105 / 99), 8 with four (float32 16384 x 1024 24.2 / 25.9 / 25.7, 65536 x 1024 97.7 / 96.0 / 92.6).
 template <typename T, int V, int TEAM>
 static void launch_fwd(const NormFwd &p, hipStream_t s) {
     constexpr int kThreads = TEAM > 256 ? TEAM : 256;
-    const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = 2048 / (kThreads / 256);
+    const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = (V <= 2 ? 4096 : 2048) / (kThreads / 256);
     hipLaunchKernelGGL((norm_fwd_kernel<T, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
 }
 
@@ -505,7 +511,7 @@ static void launch_bwd_as(const NormBwd &p, unsigned grid, hipStream_t s) {
 template <typename T, int V, int TEAM>
 static void launch_bwd(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
     constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM;
-    const int64_t want = ceil_div(p.M, kTeams), cap = norm_bwd_parts(p.M, p.N);
+    const int64_t want = ceil_div(p.M, kTeams), cap = norm_bwd_parts(p.M, p.N, sizeof(T) == 2);
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     *parts = grid;
     if (grid == 1) {            // a single workgroup's sums are the gradients
