@@ -58,6 +58,9 @@ class CModel:
     def __init__(self, cfg, batch, rank=0, world=1, comm=None, table_owner=None, seed=0, force_exchange=False,
                  overlap=-1, presort=1, wgrad_stream=-1, idx_dtype=torch.int32, device="cuda", gemm_mode=0,
                  one_id_per_bag=False, graph_steps=False, comm_dense=None):
+        if cfg.norm or cfg.keep8:
+            raise ValueError("the C-hosted step has no normalised layers (norm) and no 8-bit checkpoints (keep8): "
+                             "use dlrm_amd.model.DLRM")
         self.L = _capi.lib()
         self.cfg, self.B, self.rank, self.world = cfg, batch, rank, world
         self.dev = torch.device(device)

@@ -201,3 +201,12 @@ def test_reference_checkpoint():
     low = (exps[6:].long() > 1)
     blocks = torch.nn.functional.pad(v[6:].abs(), (0, 26)).view(44, 3, 32).amax(2)
     assert (blocks >= 63.75 * torch.pow(2.0, (exps[6:].long() - 127).double()))[low].all()
+
+
+@pytest.mark.parametrize("option", [dict(norm=True), dict(keep8=True)])
+def test_the_c_hosted_model_refuses(option):
+    """The step hosted in C has neither: it must not train another model than the one asked for."""
+    from dlrm_amd.cmodel import CModel
+    from dlrm_amd.model import DLRMConfig
+    with pytest.raises(ValueError, match="C-hosted"):
+        CModel(DLRMConfig.mlperf(**option), 64)
