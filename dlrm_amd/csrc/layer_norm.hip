@@ -15,7 +15,8 @@
 //
 // Measured (a 1 GiB copy reaches 5.1 to 5.4 TB/s here): forward 65536 x 1024 float32 97 us = 5.5 TB/s, with both checkpoints
 // 138 us = 4.9; backward 202 us = 5.3 TB/s from x with a mask, 124 us = 5.4 from the checkpoints; bf16 56 us = 4.8 forward,
-// 104 us = 5.2 backward from x.  Rows of 16384 float32 from a checkpoint spill (213 us, 3.2 TB/s).
+// 104 us = 5.2 backward from x.  Backward 4096 x 16384, a workgroup of 1024 threads per row: float32 216 us = 5.0 from x,
+// 146 us = 4.6 from the checkpoints; bf16 137 us = 3.9 and 109 us = 3.7 (one row in flight per compute unit).
 #include "act8.h"
 
 namespace dlrm {
@@ -314,17 +315,22 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
     int turn = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < p.M; r0 += (int64_t)gridDim.x * kTeams, turn ^= 1) {
         const bool live = r0 + team < p.M;
+        // (a lane number that the compiler has to take as new per row: what it makes from it, addresses and conditions of every
+        // piece, would otherwise be held from row to row and spill where the row takes 80 of 128 registers: 4096 x 16384 from
+        // checkpoints 211 us instead of 146)
+        int at = lane;
+        if constexpr (TEAM == 1024 && V * VEC == 16) asm volatile("" : "+v"(at));
         const int64_t row = live ? r0 + team : p.M - 1;
         const float rstd = p.rstd[row], mean = FROM8 ? 0.f : p.mean[row];
         float xh[V][VEC], d[V][VEC], s1 = 0.f, s2 = 0.f;
         NormGradPiece<T, VEC, FROM8, MASK> piece[V];
 #pragma unroll
-        for (int v = 0; v < V; v++) piece[v].request(p, row, (v * TEAM + lane) * VEC);
+        for (int v = 0; v < V; v++) piece[v].request(p, row, (v * TEAM + at) * VEC);
 #pragma unroll
-        for (int v = 0; v < V; v++) piece[v].values(p, (v * TEAM + lane) * VEC, mean, rstd, xh[v], d[v]);
+        for (int v = 0; v < V; v++) piece[v].values(p, (v * TEAM + at) * VEC, mean, rstd, xh[v], d[v]);
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            if (!kHoldGamma) param_elems<VEC>(p.gamma, (v * TEAM + lane) * VEC, p.N, g[v], 1.f);
+            if (!kHoldGamma) param_elems<VEC>(p.gamma, (v * TEAM + at) * VEC, p.N, g[v], 1.f);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 if (live) {
@@ -340,7 +346,7 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         const float c1 = s1 / (float)p.N, c2 = s2 / (float)p.N;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int c = (v * TEAM + lane) * VEC;
+            const int c = (v * TEAM + at) * VEC;
 #pragma unroll
             for (int j = 0; j < VEC; j++) d[v][j] = rstd * (d[v][j] - c1 - xh[v][j] * c2);
             if (p.dx_max && live) fold_elems<T, VEC>(d[v], c, p.N, vmax);
