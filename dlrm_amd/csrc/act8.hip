@@ -31,39 +31,42 @@ struct Act8Pass {
     int64_t rows;
     int cols, blocks;
     int lanes_log2;        // lanes that share a row: 2^lanes_log2, a wave at most
+    int chunks;            // of four steps in a row that is longer than one
 };
 
-// S: steps that a lane takes per row, 4 meaning "four at a time, as often as the row needs"; with S = 1 or 2 it takes four
-// or two rows at a time, so that four loads are in flight per lane whatever the row's width
+// S: steps that a lane takes per row, 4 meaning "four at a time": longer rows are cut into chunks of four steps
+// (blocks do not depend on one another), which spread over the grid's second axis where there are few rows: 42 x 14764
+// float32 there and back 31.6 us with a wave for a whole row, 13.3 this way (two launches from the host).  With S = 1 or 2 a
+// lane takes four or two rows at a time, so that four loads are in flight per lane whatever the row's width.
 template <typename T, int S>
 __global__ __launch_bounds__(256) void act8_pack_kernel(Act8Pass p) {
     constexpr int VEC = kWide<T>, R = 4 / S;
     const int lane = threadIdx.x & 63, lanes = 1 << p.lanes_log2;
-    const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC, width = p.blocks * kAct8Block;
+    const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC;
     const int rows_per_wave = 64 >> p.lanes_log2;
     const int64_t n_waves = (int64_t)gridDim.x * 4;
-    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave * R; r0 < p.rows; r0 += n_waves * rows_per_wave * R) {
-        // (every lane of the wave takes every turn: the exchanges inside act8_store need the neighbours)
-        for (int base = 0; base < width; base += S * step) {
-            u32x4 x[4];
-            int64_t row[R];
-            bool live[R];
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave * R; r0 < p.rows; r0 += n_waves * rows_per_wave * R)
+    for (int chunk = blockIdx.y; chunk < p.chunks; chunk += gridDim.y) {
+        // (every lane of the wave takes every step: the exchanges inside act8_store need the neighbours)
+        const int base = chunk * (S * step) + first;
+        u32x4 x[4];
+        int64_t row[R];
+        bool live[R];
 #pragma unroll
-            for (int k = 0; k < R; k++) {
-                row[k] = r0 + k * rows_per_wave + (lane >> p.lanes_log2);
-                live[k] = row[k] < p.rows;
-                if (!live[k]) row[k] = p.rows - 1;
-            }
+        for (int k = 0; k < R; k++) {
+            row[k] = r0 + k * rows_per_wave + (lane >> p.lanes_log2);
+            live[k] = row[k] < p.rows;
+            if (!live[k]) row[k] = p.rows - 1;
+        }
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                x[u] = request_elems<T, VEC>(static_cast<const T *>(p.src) + row[u / S] * p.ld, base + (u % S) * step + first, p.cols);
+        for (int u = 0; u < 4; u++)
+            x[u] = request_elems<T, VEC>(static_cast<const T *>(p.src) + row[u / S] * p.ld, base + (u % S) * step, p.cols);
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int c = base + (u % S) * step + first;
-                float v[VEC];
-                elems_of<T, VEC>(x[u], c, p.cols, v);
-                act8_store<VEC>(v, p.codes + row[u / S] * p.codes_ld, p.exps + row[u / S] * p.exps_ld, c, p.blocks, live[u / S]);
-            }
+        for (int u = 0; u < 4; u++) {
+            const int c = base + (u % S) * step;
+            float v[VEC];
+            elems_of<T, VEC>(x[u], c, p.cols, v);
+            act8_store<VEC>(v, p.codes + row[u / S] * p.codes_ld, p.exps + row[u / S] * p.exps_ld, c, p.blocks, live[u / S]);
         }
     }
 }
@@ -75,40 +78,42 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(Act8Pass p) {
     const int first = (lane & (lanes - 1)) * VEC, step = lanes * VEC;
     const int rows_per_wave = 64 >> p.lanes_log2;
     const int64_t n_waves = (int64_t)gridDim.x * 4;
-    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave * R; r0 < p.rows; r0 += n_waves * rows_per_wave * R) {
-        for (int base = first; base < p.cols; base += S * step) {
-            unsigned w[4][VEC / 4];
-            int e[4];
-            int64_t row[R];
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows_per_wave * R; r0 < p.rows; r0 += n_waves * rows_per_wave * R)
+    for (int chunk = blockIdx.y; chunk < p.chunks; chunk += gridDim.y) {
+        const int base = chunk * (S * step) + first;
+        unsigned w[4][VEC / 4];
+        int e[4];
+        int64_t row[R];
 #pragma unroll
-            for (int k = 0; k < R; k++) row[k] = r0 + k * rows_per_wave + (lane >> p.lanes_log2);
+        for (int k = 0; k < R; k++) row[k] = r0 + k * rows_per_wave + (lane >> p.lanes_log2);
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int64_t r = row[u / S] < p.rows ? row[u / S] : p.rows - 1;
-                const int c = base + (u % S) * step;
-                act8_load<VEC>(p.codes + r * p.codes_ld, c, p.blocks, w[u]);
-                e[u] = p.exps[r * p.exps_ld + min(c / kAct8Block, p.blocks - 1)];
-            }
+        for (int u = 0; u < 4; u++) {
+            const int64_t r = row[u / S] < p.rows ? row[u / S] : p.rows - 1;
+            const int c = base + (u % S) * step;
+            act8_load<VEC>(p.codes + r * p.codes_ld, c, p.blocks, w[u]);
+            e[u] = p.exps[r * p.exps_ld + min(c / kAct8Block, p.blocks - 1)];
+        }
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int c = base + (u % S) * step;
-                float v[VEC];
-                act8_values<VEC>(w[u], act8_step(e[u]), v);
-                if (c < p.cols && row[u / S] < p.rows) store_elems<T, VEC>(static_cast<T *>(p.dst) + row[u / S] * p.ld, c, p.cols, v);
-            }
+        for (int u = 0; u < 4; u++) {
+            const int c = base + (u % S) * step;
+            float v[VEC];
+            act8_values<VEC>(w[u], act8_step(e[u]), v);
+            if (c < p.cols && row[u / S] < p.rows) store_elems<T, VEC>(static_cast<T *>(p.dst) + row[u / S] * p.ld, c, p.cols, v);
         }
     }
 }
 
-// lanes per row (a block's stay together), steps of a lane per row and workgroups
-static unsigned act8_grid(Act8Pass &p, int vec, int *steps) {
+// lanes per row (a block's stay together), steps of a lane per row, chunks of a row and workgroups
+static dim3 act8_grid(Act8Pass &p, int vec, int *steps) {
     const int per_row = p.blocks * (kAct8Block / vec);
     p.lanes_log2 = vec == 8 ? 2 : 3;
     while (p.lanes_log2 < 6 && (1 << p.lanes_log2) < per_row) p.lanes_log2++;
     const int s = (per_row + (1 << p.lanes_log2) - 1) >> p.lanes_log2;
     *steps = s <= 2 ? s : 4;
+    p.chunks = (int)ceil_div(s, *steps);
     const int64_t want = ceil_div(p.rows, (int64_t)4 * (64 >> p.lanes_log2) * (4 / *steps));
-    return (unsigned)(want < 4096 ? want : 4096);
+    const unsigned gx = (unsigned)(want < 4096 ? want : 4096), gy = 4096 / gx;
+    return dim3(gx, gy < (unsigned)p.chunks ? gy : (unsigned)p.chunks);
 }
 
 static int act8_args(const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld, const dlrm_act8 *a) {
@@ -135,10 +140,10 @@ using namespace dlrm;
 #define DLRM_ACT8_LAUNCH(KERNEL, T)                                                                       \
     do {                                                                                                  \
         int steps = 1;                                                                                    \
-        const unsigned grid = act8_grid(p, kWide<T>, &steps);                                             \
-        if (steps == 1) hipLaunchKernelGGL((KERNEL<T, 1>), dim3(grid), dim3(256), 0, as_stream(stream), p);      \
-        else if (steps == 2) hipLaunchKernelGGL((KERNEL<T, 2>), dim3(grid), dim3(256), 0, as_stream(stream), p); \
-        else hipLaunchKernelGGL((KERNEL<T, 4>), dim3(grid), dim3(256), 0, as_stream(stream), p);          \
+        const dim3 grid = act8_grid(p, kWide<T>, &steps);                                             \
+        if (steps == 1) hipLaunchKernelGGL((KERNEL<T, 1>), grid, dim3(256), 0, as_stream(stream), p);      \
+        else if (steps == 2) hipLaunchKernelGGL((KERNEL<T, 2>), grid, dim3(256), 0, as_stream(stream), p); \
+        else hipLaunchKernelGGL((KERNEL<T, 4>), grid, dim3(256), 0, as_stream(stream), p);          \
         DLRM_LAUNCH_CHECK();                                                                              \
     } while (0)
 
