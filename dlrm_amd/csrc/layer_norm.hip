@@ -302,7 +302,9 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
     constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
     __shared__ float slots[2][TEAM > 64 ? kThreads / 32 : 1];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    constexpr bool kHoldGamma = TEAM < 512;     // (workgroups of 8 waves and more have no registers for it: read again per row)
+    // (workgroups of 8 waves and more have no registers for more than one piece: read again per row.  Held, one piece takes bf16
+    // 14827 x 2263 from x from 119 to 93 us)
+    constexpr bool kHoldGamma = TEAM < 512 || V == 1;
     float g[V][VEC], acc_g[V][VEC], acc_b[V][VEC];
 #pragma unroll
     for (int v = 0; v < V; v++) {
@@ -489,12 +491,16 @@ __global__ __launch_bounds__(1024) void param_sums_kernel(ParamSums p) {
 }
 
 // ---- launches.  Rows per width: a team of 8 to 64 lanes with up to 32 elements a lane, then 256 and 1024 threads.
-// Most partial rows that a backward launch leaves, which are its workgroups: two per compute unit (us from x, float32:
-// 8192 x 512 14.0 with 512 workgroups, 15.6 with 256, 14.4 with 1024; 8192 x 1024 21.7, 24.3, 23.7).  Requesting the next
-// row ahead of a row's sums was measured at no gain (14.1, 21.9): other waves cover the wait.  bf16 rows up to 2048 have one
-// piece a lane in flight and take four per compute unit (65536 x 1024 from x 104 against 142 us, 8192 x 1024 20.2 against
-// 21.0; 2048: 117 us; 16384 x 4096 127 against 122 with two).
-static int64_t norm_bwd_cap(int N, bool bf16) { return N <= 2048 && bf16 ? 1024 : N <= 8192 ? 512 : (N <= kLongRow ? 256 : 64); }
+// Most partial rows that a backward launch leaves, which are its workgroups (us for 256 / 512 / 1024).  Rows of one piece a
+// lane, in workgroups of 256 threads, take four per compute unit: float32 131072 x 256 165 / 102 / 106 from x, 146 / 86 / 67
+// from checkpoints, bf16 65536 x 1024 from x 142 with 512, 104 with 1024.  More pieces or threads fill it with two: float32
+// 8192 x 1024 from x 24.3 / 21.7 / 23.7, bf16 8192 x 4096 79 / 61 / 66, and beyond 4096 columns with one: float32 4096 x 8192
+// 112 / 119 / 129, bf16 61 / 66 / 81, 624 x 6714 20 / 25 / 31.  Requesting the next row ahead of a row's sums gained nothing
+// to 7 % from x and cost as much from checkpoints: other waves cover the wait.
+static int64_t norm_bwd_cap(int N, bool bf16) {
+    if (N > kLongRow) return 64;
+    return N <= (bf16 ? 2048 : 256) ? 1024 : N <= 4096 ? 512 : 256;
+}
 static int64_t norm_bwd_parts(int64_t M, int N, bool bf16 = true) {        // (a workspace holds either type's)
     const int64_t cap = norm_bwd_cap(N, bf16);
     return M < cap ? (M < 1 ? 1 : M) : cap;
