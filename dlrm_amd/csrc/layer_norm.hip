@@ -506,13 +506,16 @@ static int64_t norm_bwd_parts(int64_t M, int N, bool bf16 = true) {        // (a
     return M < cap ? (M < 1 ? 1 : M) : cap;
 }
 
-// Forward workgroups of 256 threads at most, each with several rows: 16 per compute unit where a lane has one or two pieces
-// (us, 2048 / 4096 / 8192 workgroups: bf16 65536 x 1024 66.6 / 56.2 / 56.7, 32768 x 512 16.6 / 16.2 / 18.2, float32
-// 262144 x 256 120 / 105 / 99), 8 with four (float32 16384 x 1024 24.2 / 25.9 / 25.7, 65536 x 1024 97.7 / 96.0 / 92.6).
+// Forward workgroups at most (of 256 threads; fewer of more), each with several rows: 16 per compute unit, 8 where a lane has
+// four pieces of float32 (us, 2048 / 4096 / 8192 workgroups: bf16 65536 x 1024 66.6 / 56.2 / 56.7, 32768 x 512 16.6 / 16.2 /
+// 18.2, float32 262144 x 256 120 / 105 / 99; 16384 x 1024 24.2 / 25.9 / 25.7, 65536 x 1024 97.7 / 96.0 / 92.6).  Lanes with 16
+// elements have the registers for 4 workgroups at a time, and a second round that is not full costs more than second
+// rows do: 8160 x 514 float32 16.1 us with 2040 workgroups, 13.6 with 1024, 349 x 12000 14.7 and 12.4.
 template <typename T, int V, int TEAM>
 static void launch_fwd(const NormFwd &p, hipStream_t s) {
-    constexpr int kThreads = TEAM > 256 ? TEAM : 256;
-    const int64_t want = ceil_div(p.M, kThreads / TEAM), cap = (V <= 2 ? 4096 : 2048) / (kThreads / 256);
+    constexpr int kThreads = TEAM > 256 ? TEAM : 256, kAtOnce = 1024 / (kThreads / 256);
+    const int64_t want = ceil_div(p.M, kThreads / TEAM);
+    const int64_t cap = V * kWide<T> == 16 && want <= 2 * kAtOnce ? kAtOnce : (V <= 2 ? 4 : 2) * kAtOnce;
     hipLaunchKernelGGL((norm_fwd_kernel<T, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
 }
 
