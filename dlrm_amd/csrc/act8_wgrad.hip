@@ -288,32 +288,44 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
         }
 }
 
-// Tile and ranges.  The widest tile that still gives 256 workgroups with at least 512 rows each is taken, cut into ranges
-// until there are 512 workgroups (two per compute unit, measured below against one and four); what is smaller gets 64 x 64
-// tiles and 256 workgroups.  Measured (us; tile, workgroups): 65536 x 1024 x 1024 339 (128x256, 512), 409 (256), 361 (1024),
-// 407 (128x128, 512); 8192 x 512 x 1024 39.3 (128x256, 256), 41.4 (64x128, 768); 8192 x 256 x 512 22.2 (64x128, 256),
-// 24.6 (128x128, 256); 8192 x 128 x 256 12.2 (64x64, 256), 13.9 (128x64, 256); 512 x 1024 x 1024 12.8 (64x64, 256), 17.3 (512).
+// Tile and ranges: the least of a model of the time over the four tiles, each with the ranges that give about 256, 512, 768 or
+// 1024 workgroups.  A step of 16 rows takes a workgroup `alone` us; at_once of them share a compute unit and then take
+// `each` us of it apiece, their tiles are stored at 5 outputs a ns, and the addition of the ranges is a launch and 4 bytes an
+// output and range at 4.2 TB/s.  The constants are a fit to 1100 measured pairs of tile and ranges (60 shapes, 512 to 65536
+// rows, 1 to 1024 columns; 5 % root mean square near a shape's best), and what the model takes is 2 % slower on average than
+// the fastest of a shape's pairs, 14 % at most.  Taking the widest tile that fills 512 workgroups was 17 % slower on average:
+// 53205 x 720 x 34 61 us with 128 x 256 tiles, 34 with 64 x 64; 25089 x 679 x 143 56 us with 294 workgroups of 128 x 256, 45
+// with 759 of 64 x 64; 11515 x 643 x 255 39 and 30.
 Wgrad8Shape wgrad8_shape(int64_t M, int N, int K, size_t max_bytes) {
-    static const struct { int tm, tn; int64_t want, depth; } tiles[4] = {{128, 256, 512, 512}, {128, 128, 512, 512}, {64, 128, 512, 512}, {64, 64, 256, 256}};
-    int64_t s = 1;
-    int pick = 3;
-    for (int i = 0; i < 4; i++) {
-        const int64_t n = ceil_div(N, tiles[i].tm) * ceil_div(K, tiles[i].tn);
-        s = ceil_div(tiles[i].want, n);
-        s = s > M / tiles[i].depth ? M / tiles[i].depth : s;
-        s = s < 1 ? 1 : (s > 256 ? 256 : s);
-        pick = i;
-        // (a tile that N or K fills to no more than half leaves the other half of its work to columns that do not exist)
-        if (n * s >= 256 && (tiles[i].tm == 64 || 2 * N > tiles[i].tm) && (tiles[i].tn == 64 || 2 * K > tiles[i].tn)) break;
-    }
-    const size_t slab = sizeof(float) * ((size_t)N * K + N);
-    if (max_bytes != 0 && (size_t)s * slab > max_bytes) s = max_bytes < 2 * slab ? 1 : (int64_t)(max_bytes / slab);
+    static const struct { int tm, tn; float alone, each; int at_once; } tiles[4] = {
+        {128, 256, .74f, .58f, 2}, {128, 128, .48f, .375f, 2}, {64, 128, .28f, .225f, 3}, {64, 64, .21f, .145f, 4}};
+    const int64_t rows_in = M < 1 ? 1 : M, unit = (int64_t)N * K + N;
+    const size_t slab = sizeof(float) * (size_t)unit;
+    int64_t most = rows_in / 64 < 1 ? 1 : (rows_in / 64 > 256 ? 256 : rows_in / 64);
+    if (max_bytes != 0 && (size_t)most * slab > max_bytes) most = max_bytes < 2 * slab ? 1 : (int64_t)(max_bytes / slab);
     Wgrad8Shape w{};
-    w.tm = tiles[pick].tm;
-    w.tn = tiles[pick].tn;
-    const int64_t rows = ceil_div(ceil_div(M < 1 ? 1 : M, s), 32) * 32;
-    w.rows_per_split = (int)rows;
-    w.splits = (int)ceil_div(M < 1 ? 1 : M, rows);
+    float least = 0.f;
+    for (const auto &t : tiles) {
+        const int64_t n = ceil_div(N, t.tm) * ceil_div(K, t.tn);
+        for (int want = 256; want <= 1024; want += 256) {
+            int64_t s = (want + n / 2) / n;
+            s = s < 1 ? 1 : (s > most ? most : s);
+            const int64_t rows = ceil_div(ceil_div(rows_in, s), 32) * 32;
+            s = ceil_div(rows_in, rows);
+            const int64_t wave = 256 * t.at_once, left = n * s % wave;
+            float step = (float)(n * s / wave) * t.each * t.at_once;        // us that one step of all workgroups takes
+            if (left > 0) step += fmaxf(t.alone, t.each * (float)ceil_div(left, 256));
+            const float us = step * (float)(rows / kStepRows) + 2e-7f * (float)((n * s < wave ? n * s : wave) * t.tm * t.tn) +
+                             (s > 1 ? 4.f + (float)(s * unit) * 0.95e-6f : 0.f);
+            if (w.splits == 0 || us < least) {
+                least = us;
+                w.tm = t.tm;
+                w.tn = t.tn;
+                w.splits = (int)s;
+                w.rows_per_split = (int)rows;
+            }
+        }
+    }
     w.bytes = w.splits * slab + 256;
     return w;
 }
