@@ -57,6 +57,18 @@ struct NormBwd {
     int N;
 };
 
+// Teams of 256 lanes and more are a workgroup of as many waves as the row needs, TEAM lanes at most; the sums of waves that
+// it does not have are zeros from the start.  bf16, us with a power of two of waves and with those that the row needs: 6672 x
+// 5029 forward 61.5, 47.1, 14827 x 2263 backward from x 93.7, 75.6, 32577 x 1030 91.6, 79.2.
+template <int TEAM>
+__device__ inline int team_lanes() { return TEAM >= 256 ? (int)blockDim.x : TEAM; }
+template <int TEAM, int SLOTS>
+__device__ inline void clear_slots(float (&slots)[2][SLOTS]) {
+    if constexpr (TEAM >= 256) {
+        if (threadIdx.x < 2 * SLOTS) slots[threadIdx.x / SLOTS][threadIdx.x % SLOTS] = 0.f;
+        __syncthreads();
+    }
+}
 // sum over the TEAM lanes that share a row, the same bits in all of them.  Teams of several waves meet in `slot` (a float
 // for each wave of the workgroup): the caller alternates between slots, so that a slot is written again only behind a later barrier.
 template <int TEAM>
@@ -159,11 +171,12 @@ template <typename T, int V, int TEAM>
 __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(NormFwd p) {
     constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
     __shared__ float slots[2][TEAM > 64 ? kThreads / 64 : 1];
-    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int lanes = team_lanes<TEAM>(), lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    clear_slots<TEAM>(slots);
     float g[V][VEC], b[V][VEC];
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const int c = (v * TEAM + lane) * VEC;
+        const int c = (v * lanes + lane) * VEC;
         param_elems<VEC>(p.gamma, c, p.N, g[v], 1.f);
         param_elems<VEC>(p.beta, c, p.N, b[v], 0.f);
     }
@@ -175,9 +188,9 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(Nor
         u32x4 raw[V];
         float x[V][VEC], s = 0.f, q = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; v++) raw[v] = request_elems<T, VEC>(xr, (v * TEAM + lane) * VEC, p.N);
+        for (int v = 0; v < V; v++) raw[v] = request_elems<T, VEC>(xr, (v * lanes + lane) * VEC, p.N);
 #pragma unroll
-        for (int v = 0; v < V; v++) elems_of<T, VEC>(raw[v], (v * TEAM + lane) * VEC, p.N, x[v]);
+        for (int v = 0; v < V; v++) elems_of<T, VEC>(raw[v], (v * lanes + lane) * VEC, p.N, x[v]);
 #pragma unroll
         for (int v = 0; v < V; v++)
 #pragma unroll
@@ -187,11 +200,11 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(Nor
         for (int v = 0; v < V; v++)
 #pragma unroll
             for (int j = 0; j < VEC; j++) x[v][j] -= mean;
-        if (p.N < V * TEAM * VEC) {        // (uniform: a row that fills its team has no columns to take out)
+        if (p.N < V * lanes * VEC) {        // (uniform: a row that fills its team has no columns to take out)
 #pragma unroll
             for (int v = 0; v < V; v++)
 #pragma unroll
-                for (int j = 0; j < VEC; j++) x[v][j] = (v * TEAM + lane) * VEC + j < p.N ? x[v][j] : 0.f;
+                for (int j = 0; j < VEC; j++) x[v][j] = (v * lanes + lane) * VEC + j < p.N ? x[v][j] : 0.f;
         }
 #pragma unroll
         for (int v = 0; v < V; v++)
@@ -207,7 +220,7 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_fwd_kernel(Nor
 #pragma unroll
             for (int j = 0; j < VEC; j++) x[v][j] *= rstd;
             float top = 0.f;
-            norm_output<T, VEC>(p, row, (v * TEAM + lane) * VEC, live, x[v], g[v], b[v], top);
+            norm_output<T, VEC>(p, row, (v * lanes + lane) * VEC, live, x[v], g[v], b[v], top);
             if (live) vmax = fmaxf(vmax, top);      // (y may be x: a team without a row may have read a finished one)
         }
     }
@@ -301,14 +314,15 @@ template <typename T, int V, int TEAM, bool FROM8, int MASK>
 __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(NormBwd p) {
     constexpr int VEC = kWide<T>, kThreads = TEAM > 256 ? TEAM : 256, kTeams = kThreads / TEAM;
     __shared__ float slots[2][TEAM > 64 ? kThreads / 32 : 1];
-    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int lanes = team_lanes<TEAM>(), lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    clear_slots<TEAM>(slots);
     // (workgroups of 8 waves and more have no registers for more than one piece: read again per row.  Held, one piece takes bf16
     // 14827 x 2263 from x from 119 to 93 us)
     constexpr bool kHoldGamma = TEAM < 512 || V == 1;
     float g[V][VEC], acc_g[V][VEC], acc_b[V][VEC];
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const int c = (v * TEAM + lane) * VEC;
+        const int c = (v * lanes + lane) * VEC;
         if (kHoldGamma) param_elems<VEC>(p.gamma, c, p.N, g[v], 1.f);
 #pragma unroll
         for (int j = 0; j < VEC; j++) acc_g[v][j] = acc_b[v][j] = 0.f;
@@ -327,12 +341,12 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         float xh[V][VEC], d[V][VEC], s1 = 0.f, s2 = 0.f;
         NormGradPiece<T, VEC, FROM8, MASK> piece[V];
 #pragma unroll
-        for (int v = 0; v < V; v++) piece[v].request(p, row, (v * TEAM + at) * VEC);
+        for (int v = 0; v < V; v++) piece[v].request(p, row, (v * lanes + at) * VEC);
 #pragma unroll
-        for (int v = 0; v < V; v++) piece[v].values(p, (v * TEAM + at) * VEC, mean, rstd, xh[v], d[v]);
+        for (int v = 0; v < V; v++) piece[v].values(p, (v * lanes + at) * VEC, mean, rstd, xh[v], d[v]);
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            if (!kHoldGamma) param_elems<VEC>(p.gamma, (v * TEAM + at) * VEC, p.N, g[v], 1.f);
+            if (!kHoldGamma) param_elems<VEC>(p.gamma, (v * lanes + at) * VEC, p.N, g[v], 1.f);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 if (live) {
@@ -348,7 +362,7 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         const float c1 = s1 / (float)p.N, c2 = s2 / (float)p.N;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int c = (v * TEAM + at) * VEC;
+            const int c = (v * lanes + at) * VEC;
 #pragma unroll
             for (int j = 0; j < VEC; j++) d[v][j] = rstd * (d[v][j] - c1 - xh[v][j] * c2);
             if (p.dx_max && live) fold_elems<T, VEC>(d[v], c, p.N, vmax);
@@ -381,7 +395,7 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
     } else {
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int c = (v * TEAM + lane) * VEC;
+            const int c = (v * lanes + lane) * VEC;
             if (p.part_g) store_sums<VEC>(p.part_g + (int64_t)blockIdx.x * p.part_stride, c, p.N, acc_g[v]);
             if (p.part_b) store_sums<VEC>(p.part_b + (int64_t)blockIdx.x * p.part_stride, c, p.N, acc_b[v]);
         }
@@ -490,38 +504,49 @@ __global__ __launch_bounds__(1024) void param_sums_kernel(ParamSums p) {
     }
 }
 
-// ---- launches.  Rows per width: a team of 8 to 64 lanes with up to 32 elements a lane, then 256 and 1024 threads.
-// Most partial rows that a backward launch leaves, which are its workgroups (us for 256 / 512 / 1024).  Rows of one piece a
-// lane, in workgroups of 256 threads, take four per compute unit: float32 131072 x 256 165 / 102 / 106 from x, 146 / 86 / 67
-// from checkpoints, bf16 65536 x 1024 from x 142 with 512, 104 with 1024.  More pieces or threads fill it with two: float32
-// 8192 x 1024 from x 24.3 / 21.7 / 23.7, bf16 8192 x 4096 79 / 61 / 66, and beyond 4096 columns with one: float32 4096 x 8192
-// 112 / 119 / 129, bf16 61 / 66 / 81, 624 x 6714 20 / 25 / 31.  Requesting the next row ahead of a row's sums gained nothing
-// to 7 % from x and cost as much from checkpoints: other waves cover the wait.
+// ---- launches.
+static int row_threads(int N, int elems) { return (int)ceil_div(N, 64 * elems) * 64; }
+
+// Most partial rows that a backward launch leaves, which are its workgroups: as many whole ones as give a compute unit 1024
+// threads, or 512 where a lane has more than one piece of float32 (us for 256 / 512 / 1024 workgroups): of 256 threads, float32
+// 131072 x 256 165 / 102 / 106 from x, 146 / 86 / 67 from checkpoints, 8192 x 1024 from x 24.3 / 21.7 / 23.7, bf16 65536 x
+// 1024 from x 142 with 512, 104 with 1024; of 512, bf16 8192 x 4096 79 / 61 / 66, float32 4096 x 8192 112 / 119 / 129; of 1024,
+// bf16 61 / 66 / 81.  Requesting the next row ahead of a row's sums gained nothing to 7 % from x and cost as much from
+// checkpoints: other waves cover the wait.
 static int64_t norm_bwd_cap(int N, bool bf16) {
     if (N > kLongRow) return 64;
-    return N <= (bf16 ? 2048 : 256) ? 1024 : N <= 4096 ? 512 : 256;
+    const int threads = N <= (bf16 ? 1024 : 2048) ? 256 : row_threads(N, bf16 && N <= 8192 ? 8 : 16);
+    return 256 * ((!bf16 && N > 256 && N <= 8192 ? 512 : 1024) / threads);
 }
-static int64_t norm_bwd_parts(int64_t M, int N, bool bf16 = true) {        // (a workspace holds either type's)
+static int64_t norm_bwd_parts(int64_t M, int N, bool bf16) {
     const int64_t cap = norm_bwd_cap(N, bf16);
     return M < cap ? (M < 1 ? 1 : M) : cap;
 }
+// ... of either type, which a workspace holds
+static int64_t norm_bwd_parts(int64_t M, int N) {
+    const int64_t a = norm_bwd_parts(M, N, false), b = norm_bwd_parts(M, N, true);
+    return a > b ? a : b;
+}
 
-// Forward workgroups at most (of 256 threads; fewer of more), each with several rows: 16 per compute unit, 8 where a lane has
-// four pieces of float32 (us, 2048 / 4096 / 8192 workgroups: bf16 65536 x 1024 66.6 / 56.2 / 56.7, 32768 x 512 16.6 / 16.2 /
-// 18.2, float32 262144 x 256 120 / 105 / 99; 16384 x 1024 24.2 / 25.9 / 25.7, 65536 x 1024 97.7 / 96.0 / 92.6).  Lanes with 16
-// elements have the registers for 4 workgroups at a time, and a second round that is not full costs more than second
+// Forward workgroups at most, each with several rows: as many as give a compute unit 4096 threads, 2048 where a lane has four
+// pieces of float32 (us, 2048 / 4096 / 8192 workgroups of 256 threads: bf16 65536 x 1024 66.6 / 56.2 / 56.7, 32768 x 512 16.6 /
+// 16.2 / 18.2, float32 262144 x 256 120 / 105 / 99; 16384 x 1024 24.2 / 25.9 / 25.7, 65536 x 1024 97.7 / 96.0 / 92.6).  Lanes
+// with 16 elements have the registers for 1024 threads at a time, and a second round that is not full costs more than second
 // rows do: 8160 x 514 float32 16.1 us with 2040 workgroups, 13.6 with 1024, 349 x 12000 14.7 and 12.4.
 template <typename T, int V, int TEAM>
 static void launch_fwd(const NormFwd &p, hipStream_t s) {
-    constexpr int kThreads = TEAM > 256 ? TEAM : 256, kAtOnce = 1024 / (kThreads / 256);
-    const int64_t want = ceil_div(p.M, kThreads / TEAM);
-    const int64_t cap = V * kWide<T> == 16 && want <= 2 * kAtOnce ? kAtOnce : (V <= 2 ? 4 : 2) * kAtOnce;
-    hipLaunchKernelGGL((norm_fwd_kernel<T, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(kThreads), 0, s, p);
+    // (lanes with 16 elements: 5 or 6 waves leave places free beside one another that 2 x 8 fill, 6672 x 5029 float32 73 or 78
+    // against 65 us)
+    const int threads = TEAM == 512 && V * kWide<T> == 16 ? 512 : TEAM >= 256 ? row_threads(p.N, V * kWide<T>) : 256;
+    const int64_t want = TEAM >= 256 ? p.M : ceil_div(p.M, 256 / TEAM), at_once = 256 * (1024 / threads);
+    const int64_t cap = V * kWide<T> == 16 && want <= 2 * at_once ? at_once : (V <= 2 ? 4 : 2) * at_once;
+    hipLaunchKernelGGL((norm_fwd_kernel<T, V, TEAM>), dim3((unsigned)(want < cap ? want : cap)), dim3(threads), 0, s, p);
 }
 
 template <typename T, int V, int TEAM, bool FROM8, int MASK>
 static void launch_bwd_as(const NormBwd &p, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((norm_bwd_kernel<T, V, TEAM, FROM8, MASK>), dim3(grid), dim3(TEAM > 256 ? TEAM : 256), 0, s, p);
+    const int threads = TEAM >= 256 ? row_threads(p.N, V * kWide<T>) : 256;
+    hipLaunchKernelGGL((norm_bwd_kernel<T, V, TEAM, FROM8, MASK>), dim3(grid), dim3(threads), 0, s, p);
 }
 template <typename T, int V, int TEAM>
 static void launch_bwd(NormBwd p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {

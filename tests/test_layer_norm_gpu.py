@@ -21,7 +21,9 @@ DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}      # half a step of the stored type
 SHAPES = [(1, 1), (1, 16), (3, 2), (3, 17), (5, 31), (37, 32), (65, 33), (2, 64), (1000, 128), (9, 255), (33, 479), (4, 512),
           (131, 1000), (3, 1024), (17, 1300), (2, 2048), (5, 2049), (3, 4096), (2, 5000), (3, 8192), (2, 8200), (2, 16384), (3, 16385),
-          (1, 40001)]
+          (1, 40001),
+          # workgroups of 3, 5, 6, 10, 14 and 15 waves, with more rows than workgroups
+          (1300, 1030), (1100, 1201), (770, 2263), (513, 2856), (258, 5029), (257, 6714), (259, 11167), (300, 15300)]
 
 
 def strided(v, pad, fill=7.0):
