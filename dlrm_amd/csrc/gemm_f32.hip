@@ -53,6 +53,9 @@ constexpr int RC_TILE = BM * RC_LD;        // 4608 floats
 constexpr int TILE_MAX = RC_TILE;
 constexpr int kGemmThreads = 256;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4u __attribute__((aligned(4)));      // (in memory: 16 bytes at element alignment)
+
 struct GemmParams {
     const float *A;
     int64_t lda;
@@ -88,7 +91,8 @@ __device__ inline void request_mask(const GemmParams &p, int m, int cn, float4 (
 #pragma unroll
         for (int it = 0; it < COUNT; it++) {
             const int r = m + it * STEP;
-            mk[it] = *reinterpret_cast<const float4 *>(mask + (int64_t)(r < p.M ? r : p.M - 1) * p.mask_ld + cn);
+            const f32x4 q = *reinterpret_cast<const f32x4u *>(mask + (int64_t)(r < p.M ? r : p.M - 1) * p.mask_ld + cn);
+            mk[it] = make_float4(q[0], q[1], q[2], q[3]);
         }
         return;
     }
@@ -204,8 +208,6 @@ __device__ inline void store_output(const GemmParams &p, const f32x16 (&acc)[MI]
     constexpr int RPI = 64 / LPR;         // rows per iteration
     float *ct = ct_all + wave * (32 * CT_LD);
     const int cn = n0 + wc * (32 * NI) + (lane % LPR) * 4;
-    const bool c_vec = (reinterpret_cast<uintptr_t>(C) % 16 == 0) && (p.ldc % 4 == 0) &&
-                       (p.mask == nullptr || ((reinterpret_cast<uintptr_t>(p.mask) % 16 == 0) && (p.mask_ld % 4 == 0)));
     float vmax = 0.f;     // largest magnitude this lane stores (for c_max)
     float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.bias) {
@@ -219,7 +221,7 @@ __device__ inline void store_output(const GemmParams &p, const f32x16 (&acc)[MI]
         // the mask pieces of this row block are requested before the block is parked, so that they travel while the
         // accumulators go through LDS (one round trip to memory per block instead of one per group of rows)
         float4 mk[32 / RPI];
-        const bool mask_vec = p.mask != nullptr && c_vec && cn + 3 < p.N;
+        const bool mask_vec = p.mask != nullptr && cn + 3 < p.N;
         if (mask_vec) request_mask<32 / RPI, RPI>(p, m0 + wr * (32 * MI) + mi * 32 + (lane / LPR), cn, mk);
 #pragma unroll
         for (int ni = 0; ni < NI; ni++)
@@ -237,13 +239,13 @@ __device__ inline void store_output(const GemmParams &p, const f32x16 (&acc)[MI]
             if (p.relu) { v.x = fmaxf(v.x, 0.f); v.y = fmaxf(v.y, 0.f); v.z = fmaxf(v.z, 0.f); v.w = fmaxf(v.w, 0.f); }
             if (m >= p.M || cn >= p.N) continue;
             float *dst = C + (int64_t)m * p.ldc + cn;
-            if (c_vec && cn + 3 < p.N) {
+            if (cn + 3 < p.N) {      // (16 bytes at element alignment)
                 if (mask_vec) {
                     const float4 k = mk[it];
                     v.x = k.x > 0.f ? v.x : 0.f; v.y = k.y > 0.f ? v.y : 0.f;
                     v.z = k.z > 0.f ? v.z : 0.f; v.w = k.w > 0.f ? v.w : 0.f;
                 }
-                *reinterpret_cast<float4 *>(dst) = v;
+                *reinterpret_cast<f32x4u *>(dst) = f32x4{v.x, v.y, v.z, v.w};
                 vmax = fmaxf(fmaxf(vmax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
             } else {
                 const float e[4] = {v.x, v.y, v.z, v.w};
@@ -417,7 +419,6 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 // Workgroup tiles.  TM x TN outputs per 256-thread workgroup, TM, TN in {128, 64}; the four waves sit 2 x 2
@@ -1204,8 +1205,6 @@ __device__ inline void store_output16(const GemmParams &p, const f32x4 (&acc)[2]
     constexpr int CT_LD = 64 + 4, LPR = 16, RPI = 4;
     float *ct = ct_all + wave * (32 * CT_LD);
     const int cn = n0 + (lane % LPR) * 4;
-    const bool c_vec = (reinterpret_cast<uintptr_t>(p.C) % 16 == 0) && (p.ldc % 4 == 0) &&
-                       (p.mask == nullptr || ((reinterpret_cast<uintptr_t>(p.mask) % 16 == 0) && (p.mask_ld % 4 == 0)));
     float vmax = 0.f;
     float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.bias) {
@@ -1215,7 +1214,7 @@ __device__ inline void store_output16(const GemmParams &p, const f32x4 (&acc)[2]
         if (cn + 3 < p.N) bv.w = p.bias[cn + 3];
     }
     float4 mk[32 / RPI];
-    const bool mask_vec = p.mask != nullptr && c_vec && cn + 3 < p.N;
+    const bool mask_vec = p.mask != nullptr && cn + 3 < p.N;
     if (mask_vec) request_mask<32 / RPI, RPI>(p, m0 + wave * 32 + (lane / LPR), cn, mk);
 #pragma unroll
     for (int m = 0; m < 2; m++)
@@ -1234,13 +1233,13 @@ __device__ inline void store_output16(const GemmParams &p, const f32x4 (&acc)[2]
         if (p.relu) { v.x = fmaxf(v.x, 0.f); v.y = fmaxf(v.y, 0.f); v.z = fmaxf(v.z, 0.f); v.w = fmaxf(v.w, 0.f); }
         if (m >= p.M || cn >= p.N) continue;
         float *dst = p.C + (int64_t)m * p.ldc + cn;
-        if (c_vec && cn + 3 < p.N) {
+        if (cn + 3 < p.N) {      // (16 bytes at element alignment)
             if (mask_vec) {
                 const float4 k = mk[it];
                 v.x = k.x > 0.f ? v.x : 0.f; v.y = k.y > 0.f ? v.y : 0.f;
                 v.z = k.z > 0.f ? v.z : 0.f; v.w = k.w > 0.f ? v.w : 0.f;
             }
-            *reinterpret_cast<float4 *>(dst) = v;
+            *reinterpret_cast<f32x4u *>(dst) = f32x4{v.x, v.y, v.z, v.w};
             vmax = fmaxf(fmaxf(vmax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
         } else {
             const float e[4] = {v.x, v.y, v.z, v.w};
