@@ -5,7 +5,7 @@
 //              dx = rstd (gamma d - c1 - xh c2),  dgamma = sum over rows of d xh,  dbeta = sum over rows of d
 //
 // Both are bound by memory, so a row is read once: a team of lanes holds it in registers between the sums and the output
-// (8 to 64 lanes of a wave for rows up to 1024 float32 or 512 bf16 elements, 128 to 1024 threads up to 16384).  Deviations
+// (4 to 64 lanes of a wave for rows up to 1024 float32 or 512 bf16 elements, 128 to 1024 threads up to 16384).  Deviations
 // are squared after the mean is known, not as sum x^2 - N mean^2, which loses everything when the mean is large.  Statistics and
 // sums are float32 whatever the activation's type.  Longer rows are read again for every sum (the *_long kernels).
 //
@@ -599,10 +599,13 @@ static void launch_bwd_long(NormBwd p, float *dgamma, float *dbeta, int64_t *par
 
 // One team shape per width: the smallest that holds the row with up to 16 float32 or 8 bf16 elements a lane.  More elements
 // cost registers and with them waves in flight: bf16 backward 65536 x 1024 from x 168 us with 16 a lane, 104 us with 8.
-#define DLRM_NORM_SHAPES(T, N, CALL, LONG, ...)                                \
+// Four lanes where nothing needs the 8 lanes of a float32 checkpoint's block together (HALF): 4194304 x 16 forward
+// float32 109 us with 4, 154 with 8, bf16 94 and 164, its backward from x 142 and 249.
+#define DLRM_NORM_SHAPES(T, N, HALF, CALL, LONG, ...)                          \
     do {                                                                       \
         constexpr int W = kWide<T>, F = W / 4;                                 \
-        if ((N) <= 8 * W) CALL<T, 1, 8>(__VA_ARGS__);                          \
+        if ((N) <= 4 * W && (HALF)) CALL<T, 1, 4>(__VA_ARGS__);                \
+        else if ((N) <= 8 * W) CALL<T, 1, 8>(__VA_ARGS__);                          \
         else if ((N) <= 16 * W) CALL<T, 1, 16>(__VA_ARGS__);                   \
         else if ((N) <= 32 * W) CALL<T, 1, 32>(__VA_ARGS__);                   \
         else if ((N) <= 64 * W) CALL<T, 1, 64>(__VA_ARGS__);                   \
@@ -622,11 +625,12 @@ static void launch_fwd_long(const NormFwd &p, hipStream_t s) {
 
 template <typename T>
 static void norm_fwd(const NormFwd &p, hipStream_t s) {
-    DLRM_NORM_SHAPES(T, p.N, launch_fwd, launch_fwd_long, p, s);
+    const bool half = sizeof(T) == 2 || (p.xhat8.d_codes == nullptr && p.y8.d_codes == nullptr);
+    DLRM_NORM_SHAPES(T, p.N, half, launch_fwd, launch_fwd_long, p, s);
 }
 template <typename T>
 static void norm_bwd(const NormBwd &p, float *dgamma, float *dbeta, int64_t *parts, hipStream_t s) {
-    DLRM_NORM_SHAPES(T, p.N, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
+    DLRM_NORM_SHAPES(T, p.N, true, launch_bwd, launch_bwd_long, p, dgamma, dbeta, parts, s);
 }
 
 static bool rows_aligned(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
