@@ -172,8 +172,8 @@ __device__ inline u32x4 request_elems(const T *row, int c, int N) {
 }
 template <typename T, int VEC>
 __device__ inline void elems_of(u32x4 w, int c, int N, float (&v)[VEC], float fill = 0.f) {
-    if (N % VEC != 0) {         // (a uniform branch: rows of whole pieces skip it)
-        const int back = N >= VEC ? max(c - (N - VEC), 0) : c;
+    if (c + VEC > N && N % VEC != 0) {         // (waves without the end of the row skip it)
+        const int back = N >= VEC ? c - (N - VEC) : c;
         if constexpr (sizeof(T) == 2)
             if (back & 1) {
 #pragma unroll
