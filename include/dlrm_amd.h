@@ -393,8 +393,8 @@ int dlrm_sgd_step(float *d_w, const float *d_g, int64_t n, float lr, dlrm_stream
  *   mean = sum x / N,  rstd = 1 / sqrt(sum (x - mean)^2 / N + eps),  xh = (x - mean) rstd,  y = act(gamma xh + beta)
  *
  * x and y are DLRM_F32 or DLRM_BF16 (`dtype`); statistics and arithmetic are float32, y is rounded once.  Any row
- * stride is accepted, no element behind column N-1 is read or written, and d_y may be d_x itself; rows on 16-byte
- * boundaries take 16-byte loads and stores.  DLRM_ACT_RELU passes a NaN on.
+ * stride is accepted, no element behind column N-1 is read or written, and d_y may be d_x itself.  DLRM_ACT_RELU passes
+ * a NaN on.
  * What the backward pass needs can leave with the same pass: the statistics, the checkpoint of xh (xhat8) and that of
  * the stored y (y8, equal to what dlrm_act8_pack makes of y); each is skipped where its pointer is NULL.
  */
