@@ -36,7 +36,7 @@ struct Wgrad8 {
     int64_t ldc, slab_stride;
     float *colsum;           // or NULL
     int M, N, K;
-    int rows_per_split;      // a multiple of 32
+    int rows_per_split;      // a multiple of 32, or all rows
     int gx, gy, gz;          // gz: ranges; gx, gy are filled in by the launch
 };
 int launch_wgrad8(Wgrad8 p, int tm, int tn, hipStream_t s);

@@ -89,8 +89,8 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8 p) {
     const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (lin >> 3);
     const int bx = tile % p.gx, by = (tile / p.gx) % p.gy, bz = tile / (p.gx * p.gy);
     const int n0 = by * TM, k0 = bx * TN;
-    const int begin = bz * p.rows_per_split, end = min(p.M, begin + p.rows_per_split);
-    const int full = (end - begin) / kStepRows, steps = (end - begin + kStepRows - 1) / kStepRows;
+    const int begin = bz * p.rows_per_split, end = begin + min(p.M - begin, p.rows_per_split);    // (no sum passes M < 2^31)
+    const int full = (end - begin) / kStepRows, steps = full + ((end - begin) % kStepRows != 0);
 
     // Columns past the operands only feed outputs that are never stored: their loads are moved inside the row.  A piece of dz
     // that N cuts through is moved back too and put in its place in registers.
@@ -310,12 +310,12 @@ Wgrad8Shape wgrad8_shape(int64_t M, int N, int K, size_t max_bytes) {
         for (int want = 256; want <= 1024; want += 256) {
             int64_t s = (want + n / 2) / n;
             s = s < 1 ? 1 : (s > most ? most : s);
-            const int64_t rows = ceil_div(ceil_div(rows_in, s), 32) * 32;
+            const int64_t up = ceil_div(ceil_div(rows_in, s), 32) * 32, rows = up < rows_in ? up : rows_in;
             s = ceil_div(rows_in, rows);
             const int64_t wave = 256 * t.at_once, left = n * s % wave;
             float step = (float)(n * s / wave) * t.each * t.at_once;        // us that one step of all workgroups takes
             if (left > 0) step += fmaxf(t.alone, t.each * (float)ceil_div(left, 256));
-            const float us = step * (float)(rows / kStepRows) + 2e-7f * (float)((n * s < wave ? n * s : wave) * t.tm * t.tn) +
+            const float us = step * (float)(up / kStepRows) + 2e-7f * (float)((n * s < wave ? n * s : wave) * t.tm * t.tn) +
                              (s > 1 ? 4.f + (float)(s * unit) * 0.95e-6f : 0.f);
             if (w.splits == 0 || us < least) {
                 least = us;
