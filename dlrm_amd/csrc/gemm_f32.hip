@@ -457,6 +457,10 @@ struct TileAddr {
     unsigned off[R / 64];  // byte offsets of this thread's 16-byte pieces inside a half tile
 };
 
+// The 16-byte pieces of a tile sit at 32-bit byte offsets from its first element: whether `rows` rows `ld` elements apart, with up
+// to 128 elements of the last one, stay below 2^32 bytes (operands of longer rows are read element by element, at 64-bit addresses)
+__host__ __device__ inline bool piece_offsets_fit(int64_t ld, int rows) { return ((rows - 1) * ld + 128) * 4 <= 0xffffffffll; }
+
 template <bool RC, int R>
 __device__ inline TileAddr<RC, R> make_tile_addr(const float *base, int64_t ld, int o0, int o_end) {
     TileAddr<RC, R> t;
@@ -469,7 +473,7 @@ __device__ inline TileAddr<RC, R> make_tile_addr(const float *base, int64_t ld, 
         for (int v = 0; v < R / 64; v++) {
             const int o = o0 + (tid >> 2) + 64 * v;
             const int oc = o < o_end ? o : o_end - 1;   // surplus rows only feed outputs that are never stored
-            t.off[v] = (unsigned)((oc - o0) * (int)ld + (tid & 3) * 4) * 4u;
+            t.off[v] = ((unsigned)(oc - o0) * (unsigned)ld + (tid & 3) * 4) * 4u;
         }
     } else {
         t.origin = base + o0;
@@ -479,7 +483,7 @@ __device__ inline TileAddr<RC, R> make_tile_addr(const float *base, int64_t ld, 
         if (col >= o_end) col = o_end - 4 > o0 ? o_end - 4 : o0;
 #pragma unroll
         for (int v = 0; v < R / 64; v++)
-            t.off[v] = (unsigned)((tid / LPR + (256 / LPR) * v) * (int)ld + (col - o0)) * 4u;
+            t.off[v] = ((unsigned)(tid / LPR + (256 / LPR) * v) * (unsigned)ld + (col - o0)) * 4u;
     }
     return t;
 }
@@ -715,7 +719,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_split_kernel(GemmParams 
     // through a piece, that piece runs into the next row, so the step that holds the operand's last row is left out.
     // 16381 x 1024 x 479 with W and dx packed, dx = dz W: 215 us with 4-byte loads throughout, 117 us this way.
     auto piece_steps = [&](bool aligned, bool rc, int64_t ld, int o0, int tile, int o_end) {
-        if (ld < 4) return 0;
+        if (ld < 4 || !piece_offsets_fit(ld, rc ? tile : 16)) return 0;
         if (aligned || rc || o_end % 4 == 0 || o0 + tile <= o_end) return full_steps;
         return min(full_steps, (p.K - 1 - k_begin) / BK);
     };
@@ -825,7 +829,8 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_split_kernel(GemmParams 
         // partial last tile of reduction-contiguous operands whose rows are long enough to be read past k_end
         // (padded leading dimensions): 16-byte loads, the surplus elements zeroed in registers
         const int64_t r_hi = (int64_t)k_begin + (int64_t)steps * BK;
-        if (t_done < steps && p.a_vec && p.b_vec && r_hi <= p.lda && r_hi <= p.ldb) {
+        if (t_done < steps && p.a_vec && p.b_vec && r_hi <= p.lda && r_hi <= p.ldb && piece_offsets_fit(p.lda, TM) &&
+            piece_offsets_fit(p.ldb, TN)) {
             run(std::true_type{}, std::true_type{}, t_done, steps);
             t_done = steps;
         }
@@ -1797,7 +1802,7 @@ static int launch_f16p(GemmParams p, const dlrm_weight_planes *wp, bool transpos
                      (transposed ? (wp->N == p.K && wp->K == p.N) : (wp->N == p.N && wp->K == p.K)),
                  "w_planes do not belong to this layer's weight matrix");
     const int64_t k32 = ceil_div(p.K, 32) * 32;
-    if (!p.a_vec || (p.K % 32 != 0 && p.lda < k32)) return DLRM_OK;
+    if (!p.a_vec || (p.K % 32 != 0 && p.lda < k32) || !piece_offsets_fit(p.lda, 128)) return DLRM_OK;
     // DLRM_F16P_PATH=1 (tuning aid): both operands through registers instead of global -> LDS directly (the mixed
     // forms were measured too, all within 5 %; the kernel keeps the switches, two forms are built)
     static const int path = [] { const char *e = getenv("DLRM_F16P_PATH"); return e ? (atoi(e) != 0) : 0; }();
