@@ -122,8 +122,9 @@ class MLPStack:
 
     norm: every layer but the last is Linear + layer norm + ReLU; gamma and beta follow the layer's bias.
     keep8: what the backward pass needs of those layers waits for it in 8 bits (ops.Act8): the output, which is the next
-    layer's input and the ReLU's mask, and with norm the normalised rows.  Their float32 outputs then share two buffers
-    (hidden_buffers): a layer's is only read by the layer after it."""
+    layer's input and the ReLU's mask, and with norm the normalised rows.  Their float32 outputs then take no memory of their
+    own (hidden_buffers): a layer's is only read by the layer after it, and lies where the backward pass, which no longer needs
+    it, leaves gradients."""
 
     def __init__(self, sizes, params, grads, offset, last_relu=True, norm=False, norm_eps=1e-5, keep8=False):
         self.sizes = list(sizes)
@@ -168,13 +169,18 @@ class MLPStack:
             g.fill_(1.0)
             e.zero_()
 
-    def hidden_buffers(self, batch, device):
-        """The float32 outputs of the hidden layers ([B, N_i] views), and what the backward pass keeps of them."""
+    def gradient_buffers(self, batch, device):
+        """The pre-activation gradients of the hidden layers ([B, N_i] views)."""
+        return [torch.zeros((batch, _padk(n)), dtype=torch.float32, device=device)[:, :n] for n in self.sizes[1:-1]]
+
+    def hidden_buffers(self, batch, device, dz_bufs):
+        """The float32 outputs of the hidden layers ([B, N_i] views), and what the backward pass keeps of them.  dz_bufs: the
+        layers' gradient_buffers; with keep8 the outputs take turns in the widest of every other one of them."""
         widths = self.sizes[1:-1]
         f32 = dict(dtype=torch.float32, device=device)
         if self.keep8:
-            pair = [torch.zeros(batch * max([_padk(n) for n in widths[k::2]] or [0]), **f32) for k in (0, 1)]
-            acts = [pair[i % 2][:batch * _padk(n)].view(batch, _padk(n))[:, :n] for i, n in enumerate(widths)]
+            widest = [max(dz_bufs[k::2], key=lambda t: t.stride(0)) for k in (0, 1)[:len(widths)]]
+            acts = [widest[i % 2].as_strided((batch, n), (_padk(n), 1)) for i, n in enumerate(widths)]
             self.y8 = [ops.Act8.empty(batch, n, device) for n in widths]
             self.xhat8 = [ops.Act8.empty(batch, n, device) for n in widths] if self.norm else []
         else:
@@ -380,13 +386,13 @@ class DLRM:
             self.feat = torch.zeros((B, self.inter_ld), **f32)    # [bottom out | pooled tables], read by the top MLP
             self.dfeat = torch.zeros((B, self.inter_ld), **f32)
             self.inter, self.dinter = self.feat, self.dfeat
-        self.bot_acts = self.bottom.hidden_buffers(B, dev)
+        self.bot_dz = self.bottom.gradient_buffers(B, dev)
+        self.bot_acts = self.bottom.hidden_buffers(B, dev, self.bot_dz)
         self.bot_acts.append(self.feat[:, :cfg.bottom[-1]])
-        self.bot_dz = [torch.zeros((B, _padk(n)), **f32)[:, :n] for n in cfg.bottom[:-1]]
-        self.top_acts = self.top.hidden_buffers(B, dev)
+        self.top_dz = self.top.gradient_buffers(B, dev)
+        self.top_acts = self.top.hidden_buffers(B, dev, self.top_dz)
         self.pred = torch.zeros((B, 1), **f32)
         self.top_acts.append(self.pred)
-        self.top_dz = [torch.zeros((B, _padk(n)), **f32)[:, :n] for n in cfg.top[:-1]]
         self.dpred = torch.zeros((B, 1), **f32)
         self.loss = torch.zeros(1, **f32)
         self.ws_dense = None
