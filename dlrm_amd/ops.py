@@ -42,12 +42,17 @@ def _emit(name, *args):
 
 def _op(fn):
     """Marks a public operator: a recorder learns which operator (and with which arguments) the
-    entries recorded next belong to."""
+    entries recorded next belong to, and holds what the operator returns (outputs and workspaces that it
+    allocated itself are written by every replay)."""
     @functools.wraps(fn)
     def wrapped(*a, **kw):
-        if _recorder is not None:
-            _recorder.note(fn.__name__, a, kw)
-        return fn(*a, **kw)
+        if _recorder is None:
+            return fn(*a, **kw)
+        recorder = _recorder
+        recorder.note(fn.__name__, a, kw)
+        out = fn(*a, **kw)
+        recorder.hold(out if isinstance(out, tuple) else (out,))
+        return out
     return wrapped
 
 

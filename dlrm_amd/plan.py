@@ -92,9 +92,10 @@ class StepRecorder:
 
     def note(self, name, args, kwargs):
         self._call = (name, args, kwargs)
-        for a in list(args) + list(kwargs.values()):
-            if isinstance(a, (torch.Tensor, ops.Act8)):
-                self.plan.keep.append(a)
+        self.hold(list(args) + list(kwargs.values()))
+
+    def hold(self, values):
+        self.plan.keep += [v for v in values if isinstance(v, (torch.Tensor, ops.Act8))]
 
     def add(self, name, args):
         L = self.plan.L
