@@ -242,6 +242,13 @@ def _rows(t, what, here, shape=None):
     return st[0] if s[0] > 1 else max(st[0], s[1])
 
 
+def _f32_rows(t, what, here, shape):
+    """_rows of a float32 tensor of this shape."""
+    if t.dtype is not torch.float32:
+        raise TypeError("%s must be float32, got %s" % (what, t.dtype))
+    return _rows(t, what, here, shape)
+
+
 def _vector(t, n, what, here):
     """Address of a contiguous float32 [n] tensor on device `here` (0 for None)."""
     if t is None:
@@ -504,23 +511,29 @@ def linear_forward(x, w, bias, relu, out=None, x_absmax=None, w_absmax=None, y_a
 def linear_backward_data(dz, w, relu_mask=None, out=None, dz_absmax=None, w_absmax=None, dx_absmax=None, w_planes=None):
     """dx = dz W, optionally masked with (relu_mask > 0); relu_mask may be the Act8 of the activation.  *_absmax, w_planes: see
     linear_forward."""
-    mask8 = relu_mask if isinstance(relu_mask, Act8) else None
-    if mask8 is not None:
-        relu_mask = None
-    _require_cuda(dz, w, relu_mask, out)
-    M, N = dz.shape
-    K = w.shape[1]
-    if out is None:
-        out = torch.empty((M, K), dtype=torch.float32, device=dz.device)
-    d = _capi.LinearBwdDesc()
-    d.M, d.N, d.K = M, N, K
-    d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
-    d.d_w, d.w_ld = w.data_ptr(), _ld(w)
-    d.d_dx, d.dx_ld = out.data_ptr(), _ld(out)
-    if relu_mask is not None:
-        d.d_relu_mask, d.relu_mask_ld = relu_mask.data_ptr(), _ld(relu_mask)
-    elif mask8 is not None:
-        d.relu_mask8 = _act8(mask8, (M, K), "relu_mask", _device_of(dz))
+    if isinstance(relu_mask, Act8):
+        here = _device_of(dz)
+        d = _capi.LinearBwdDesc()
+        d.M, d.N, d.K = M, N, K = *dz.shape, relu_mask.cols
+        if out is None:
+            out = torch.empty((M, K), dtype=torch.float32, device=dz.device)
+        d.d_dz, d.dz_ld = dz.data_ptr(), _f32_rows(dz, "dz", here, (M, N))
+        d.d_w, d.w_ld = w.data_ptr(), _f32_rows(w, "w", here, (N, K))
+        d.d_dx, d.dx_ld = out.data_ptr(), _f32_rows(out, "out", here, (M, K))
+        d.relu_mask8 = _act8(relu_mask, (M, K), "relu_mask", here)
+    else:
+        _require_cuda(dz, w, relu_mask, out)
+        M, N = dz.shape
+        K = w.shape[1]
+        if out is None:
+            out = torch.empty((M, K), dtype=torch.float32, device=dz.device)
+        d = _capi.LinearBwdDesc()
+        d.M, d.N, d.K = M, N, K
+        d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
+        d.d_w, d.w_ld = w.data_ptr(), _ld(w)
+        d.d_dx, d.dx_ld = out.data_ptr(), _ld(out)
+        if relu_mask is not None:
+            d.d_relu_mask, d.relu_mask_ld = relu_mask.data_ptr(), _ld(relu_mask)
     d.gemm_mode = _gemm_field()
     d.d_dz_absmax, d.d_w_absmax, d.d_dx_absmax = _ptr0(dz_absmax), _ptr0(w_absmax), _ptr0(dx_absmax)
     if w_planes is not None:
@@ -552,27 +565,43 @@ def linear_backward_weight_workspace_bytes(M, N, K, act8=False):
     return int(n.value)
 
 
+def _wgrad8_desc(dz, x, dw, db, here):
+    """Descriptor of the weight gradient from an Act8, its tensors on device `here`."""
+    d = _capi.LinearBwdDesc()
+    d.M, d.N, d.K = M, N, K = *dz.shape, x.cols
+    d.d_dz, d.dz_ld = dz.data_ptr(), _f32_rows(dz, "dz", here, (M, N))
+    d.x8 = _act8(x, (M, K), "x", here)
+    d.d_dw, d.dw_ld = dw.data_ptr(), _f32_rows(dw, "dw", here, (N, K))
+    d.d_db = _vector(db, N, "db", here)
+    return d
+
+
 @_op
 def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True, dz_absmax=None, x_absmax=None):
     """dW = dz^T x [N,K], db = column sums of dz.  x may be the Act8 of the activation.  *_absmax: see linear_forward."""
-    x8 = x if isinstance(x, Act8) else None
-    _require_cuda(dz, x if x8 is None else None, dw, db, workspace)
+    x8 = isinstance(x, Act8)
+    if x8:
+        here = _device_of(dz)
+    else:
+        _require_cuda(dz, x, dw, db, workspace)
     M, N = dz.shape
     K = x.shape[1]
     if dw is None:
         dw = torch.empty((N, K), dtype=torch.float32, device=dz.device)
     if db is None and want_db:
         db = torch.empty((N,), dtype=torch.float32, device=dz.device)
-    need = linear_backward_weight_workspace_bytes(M, N, K, x8 is not None)
+    if x8:
+        d = _wgrad8_desc(dz, x, dw, db, here)
+        workspace, at, nbytes = _workspace(workspace, linear_backward_weight_workspace_bytes(M, N, K, True), dz, here)
+        _emit("linear_backward_weight", d, C.c_void_p(at), C.c_size_t(nbytes))
+        return dw, db, workspace
+    need = linear_backward_weight_workspace_bytes(M, N, K)
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dz.device)
     d = _capi.LinearBwdDesc()
     d.M, d.N, d.K = M, N, K
     d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
-    if x8 is not None:
-        d.x8 = _act8(x8, (M, K), "x", _device_of(dz))
-    else:
-        d.d_x, d.x_ld = x.data_ptr(), _ld(x)
+    d.d_x, d.x_ld = x.data_ptr(), _ld(x)
     d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)
     d.d_db = 0 if db is None else db.data_ptr()
     d.gemm_mode = _gemm_field()
@@ -584,20 +613,19 @@ def linear_backward_weight(dz, x, dw=None, db=None, workspace=None, want_db=True
 def linear_backward_weight_static(dz, x, dw, db=None):
     """linear_backward_weight through the entry point that allocates nothing: partial sums go to the library's
     static device array (layers beyond its size are refused); outputs must be given."""
-    x8 = x if isinstance(x, Act8) else None
-    _require_cuda(dz, x if x8 is None else None, dw, db)
-    M, N = dz.shape
-    K = x.shape[1]
-    d = _capi.LinearBwdDesc()
-    d.M, d.N, d.K = M, N, K
-    d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
-    if x8 is not None:
-        d.x8 = _act8(x8, (M, K), "x", _device_of(dz))
+    if isinstance(x, Act8):
+        d = _wgrad8_desc(dz, x, dw, db, _device_of(dz))
     else:
+        _require_cuda(dz, x, dw, db)
+        M, N = dz.shape
+        K = x.shape[1]
+        d = _capi.LinearBwdDesc()
+        d.M, d.N, d.K = M, N, K
+        d.d_dz, d.dz_ld = dz.data_ptr(), _ld(dz)
         d.d_x, d.x_ld = x.data_ptr(), _ld(x)
-    d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)
-    d.d_db = 0 if db is None else db.data_ptr()
-    d.gemm_mode = _gemm_field()
+        d.d_dw, d.dw_ld = dw.data_ptr(), _ld(dw)
+        d.d_db = 0 if db is None else db.data_ptr()
+        d.gemm_mode = _gemm_field()
     check(_capi.lib().dlrm_linear_backward_weight_static(C.byref(d), _stream()))
     return dw, db
 
