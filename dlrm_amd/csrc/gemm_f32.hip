@@ -1859,6 +1859,10 @@ static int launch_f16p(GemmParams p, const dlrm_weight_planes *wp, bool transpos
     *done = true;
     return DLRM_OK;
 }
+// Largest batch: the kernels number rows with ints, and a range's nominal end or the next row of a thread that strides over the
+// batch lies up to 2^18 rows behind the last one.
+constexpr int64_t kMostRows = (1ll << 31) - (1 << 20);
+
 // rows of an operand start on 16-byte boundaries (otherwise the kernel falls back to 4-byte loads)
 static int vec_ok(const void *p, int64_t ld) { return aligned16(p) && ld % 4 == 0; }
 
@@ -1917,7 +1921,7 @@ extern "C" int dlrm_linear_forward(const dlrm_linear *l, dlrm_stream_t stream) {
     DLRM_REQUIRE(l != nullptr, "linear descriptor is NULL");
     DLRM_REQUIRE(l->M >= 0 && l->N >= 1 && l->K >= 1, "bad shape M=%lld N=%d K=%d", (long long)l->M, l->N, l->K);
     if (l->M == 0) return DLRM_OK;
-    DLRM_REQUIRE(l->M < (1ll << 31), "M too large");
+    DLRM_REQUIRE(l->M <= kMostRows, "M too large");
     DLRM_REQUIRE(l->d_x && l->d_w && l->d_y, "NULL operand");
     DLRM_REQUIRE(l->x_ld >= l->K && l->w_ld >= l->K && l->y_ld >= l->N, "leading dimension too small");
     // the two shapes that are no matrix product: a few input columns, or one output column
@@ -1946,7 +1950,7 @@ extern "C" int dlrm_linear_backward_data(const dlrm_linear_bwd *l, dlrm_stream_t
     DLRM_REQUIRE(l != nullptr, "linear_bwd descriptor is NULL");
     DLRM_REQUIRE(l->M >= 0 && l->N >= 1 && l->K >= 1, "bad shape");
     if (l->M == 0) return DLRM_OK;
-    DLRM_REQUIRE(l->M < (1ll << 31), "M too large");
+    DLRM_REQUIRE(l->M <= kMostRows, "M too large");
     DLRM_REQUIRE(l->d_dz && l->d_w && l->d_dx, "NULL operand");
     DLRM_REQUIRE(l->dz_ld >= l->N && l->w_ld >= l->K && l->dx_ld >= l->K, "leading dimension too small");
     if (l->relu_mask8.d_codes) {
@@ -2007,8 +2011,8 @@ static int backward_weight_impl(const dlrm_linear_bwd *l, void *d_workspace, siz
     if (pending) pending->splits = 0;
     DLRM_REQUIRE(l != nullptr, "linear_bwd descriptor is NULL");
     DLRM_REQUIRE(l->M >= 1 && l->N >= 1 && l->K >= 1, "bad shape");
-    DLRM_REQUIRE(l->M < (1ll << 31), "M too large");
     const bool from8 = l->x8.d_codes != nullptr;
+    DLRM_REQUIRE(l->M <= (from8 ? (1ll << 31) - 1 : kMostRows), "M too large");
     DLRM_REQUIRE(l->d_dz && (l->d_x || from8) && l->d_dw, "NULL operand");
     DLRM_REQUIRE(!from8 || l->d_x == nullptr, "both x and its 8-bit checkpoint given");
     DLRM_REQUIRE(l->dz_ld >= l->N && (from8 || l->x_ld >= l->K) && l->dw_ld >= l->K, "leading dimension too small");

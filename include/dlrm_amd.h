@@ -277,7 +277,7 @@ int dlrm_split_weights(const dlrm_weight_planes *items, int32_t n, dlrm_stream_t
  * Layers with at most 16 inputs or a single output are no matrix product and run in one-pass float32 fma kernels.
  */
 typedef struct dlrm_linear {
-    int64_t M;          /* rows of x (batch) */
+    int64_t M;          /* rows of x (batch), at most 2^31 - 2^20 */
     int32_t N, K;       /* out features, in features */
     const float *d_x;   /* [M,K] */
     int64_t x_ld;
@@ -328,7 +328,7 @@ int dlrm_absmax(const float *d_x, int64_t rows, int32_t cols, int64_t ld, float 
  *                    Leading dimensions of dz and x8 up to 2^24.
  */
 typedef struct dlrm_linear_bwd {
-    int64_t M;
+    int64_t M;            /* at most 2^31 - 2^20; below 2^31 with x8 */
     int32_t N, K;
     const float *d_dz;  /* [M,N] */
     int64_t dz_ld;
