@@ -488,8 +488,10 @@ __device__ inline TileAddr<RC, R> make_tile_addr(const float *base, int64_t ld, 
     return t;
 }
 
-// 16-byte loads of half h of the tile whose reduction range starts at r0 (needs 16-byte aligned rows
-// and a full 32-deep tile; an RS tile must not run past the row's leading dimension)
+// 16-byte loads of half h of the tile whose reduction range starts at r0: rows at any multiple of 4 bytes, a whole 32-deep
+// tile and offsets that fit (piece_offsets_fit).  A piece of an RS tile that the operand's last column cuts through runs into
+// what follows in memory: padding up to the leading dimension, or the next row, so the last row of an operand whose rows are
+// not on 16-byte boundaries is not read this way (gemm_split_kernel: piece_steps)
 template <bool RC, int R>
 __device__ inline void load_half_vec(const TileAddr<RC, R> &t, int r0, int h, f32x4 *x) {
     // buffer loads: the wave-uniform half-tile origin travels in a scalar resource descriptor and each
@@ -717,7 +719,8 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_split_kernel(GemmParams 
     // elements; edge tiles of a reduction-strided operand read whole pieces up to the leading dimension (make_tile_addr).
     // Rows at other addresses take the same loads (buffer loads need 4-byte alignment only); where the last column cuts
     // through a piece, that piece runs into the next row, so the step that holds the operand's last row is left out.
-    // 16381 x 1024 x 479 with W and dx packed, dx = dz W: 215 us with 4-byte loads throughout, 117 us this way.
+    // 16381 x 1024 x 479 with W and dx packed, dx = dz W: 215 us with 4-byte loads throughout, 105 us this way and with 16-byte
+    // stores (padded rows: 96 us).
     auto piece_steps = [&](bool aligned, bool rc, int64_t ld, int o0, int tile, int o_end) {
         if (ld < 4 || !piece_offsets_fit(ld, rc ? tile : 16)) return 0;
         if (aligned || rc || o_end % 4 == 0 || o0 + tile <= o_end) return full_steps;
@@ -747,7 +750,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_split_kernel(GemmParams 
     };
 
     // Tiles [t_begin, t_end) of the reduction through the two-stage pipeline.  VEC: 16-byte loads
-    // (full 32-deep tiles of aligned operands), else clamped 4-byte loads with zero fill.
+    // (full 32-deep tiles, see vec_steps), else clamped 4-byte loads with zero fill.
     const TileAddr<A_RC, TM> ta = make_tile_addr<A_RC, TM>(p.A, p.lda, m0, p.M);
     const TileAddr<B_RC, TN> tb = make_tile_addr<B_RC, TN>(p.B, p.ldb, n0, p.N);
     f32x4 xa[2 * PA], xb[2 * PB], ya[2 * PA], yb[2 * PB];
@@ -835,7 +838,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_split_kernel(GemmParams 
             t_done = steps;
         }
     }
-    if (t_done < steps) run(std::false_type{}, std::false_type{}, t_done, steps);   // edge tiles, unaligned operands
+    if (t_done < steps) run(std::false_type{}, std::false_type{}, t_done, steps);   // the steps that vec_steps leaves out
 
     if constexpr (NP == 2) {      // mixed terms in, operand scales out (two exact multiplications: either factor alone stays in range)
         const float inv_a = 1.0f / scale_a, inv_b = 1.0f / scale_b;
@@ -1863,7 +1866,7 @@ static int launch_f16p(GemmParams p, const dlrm_weight_planes *wp, bool transpos
 // batch lies up to 2^18 rows behind the last one.
 constexpr int64_t kMostRows = (1ll << 31) - (1 << 20);
 
-// rows of an operand start on 16-byte boundaries (otherwise the kernel falls back to 4-byte loads)
+// rows of an operand start on 16-byte boundaries
 static int vec_ok(const void *p, int64_t ld) { return aligned16(p) && ld % 4 == 0; }
 
 // weight gradient [N,K] over a batch of M: tile and reduction split per evaluation mode

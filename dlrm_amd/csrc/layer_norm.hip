@@ -16,7 +16,9 @@
 // Measured (a 1 GiB copy reaches 5.1 to 5.4 TB/s here): forward 65536 x 1024 float32 97 us = 5.5 TB/s, with both checkpoints
 // 138 us = 4.9; backward 202 us = 5.3 TB/s from x with a mask, 124 us = 5.4 from the checkpoints; bf16 56 us = 4.8 forward,
 // 104 us = 5.2 backward from x.  Backward 4096 x 16384, a workgroup of 1024 threads per row: float32 216 us = 5.0 from x,
-// 146 us = 4.6 from the checkpoints; bf16 137 us = 3.9 and 109 us = 3.7 (one row in flight per compute unit).
+// 146 us = 4.6 from the checkpoints; bf16 137 us = 3.9 and 109 us = 3.7 (one row in flight per compute unit).  bf16 rows of
+// 1030 to 16384 columns, 33.5 million elements: forward 2.9 (6714 columns) to 5.2 TB/s (2048), backward 3.2 (5029, from
+// checkpoints) to 5.3 (2048, from x); a row takes 3 to 16 waves that meet at its sums, and what holds the slow widths was not traced.
 #include "act8.h"
 
 namespace dlrm {
@@ -333,7 +335,8 @@ __global__ __launch_bounds__((TEAM > 256 ? TEAM : 256)) void norm_bwd_kernel(Nor
         const bool live = r0 + team < p.M;
         // (a lane number that the compiler has to take as new per row: what it makes from it, addresses and conditions of every
         // piece, would otherwise be held from row to row and spill where the row takes 80 of 128 registers: 4096 x 16384 from
-        // checkpoints 211 us instead of 146)
+        // checkpoints 211 us instead of 146).  No float32 instance spills so; the four bf16 ones with a mask keep 1 to 5
+        // registers a lane in scratch.
         int at = lane;
         if constexpr (TEAM == 1024 && V * VEC == 16) asm volatile("" : "+v"(at));
         const int64_t row = live ? r0 + team : p.M - 1;

@@ -204,8 +204,8 @@ typedef struct dlrm_act8 {
 } dlrm_act8;
 
 /* A [rows, cols] activation of dtype DLRM_F32 or DLRM_BF16 into a checkpoint, and the values of a checkpoint back into
- * such a tensor (float32 and bf16 hold them exactly).  Rows may have any stride; rows on 16-byte boundaries are moved
- * 16 bytes at a time.  The packing direction writes whole blocks, the unpacking one exactly cols elements a row. */
+ * such a tensor (float32 and bf16 hold them exactly).  Any x_ld >= cols; d_x needs the alignment of its elements only.
+ * The packing direction writes whole blocks, the unpacking one exactly cols elements a row. */
 int dlrm_act8_pack(const void *d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t x_ld, const dlrm_act8 *out,
                    dlrm_stream_t stream);
 int dlrm_act8_unpack(const dlrm_act8 *a, int64_t rows, int32_t cols, void *d_x, int32_t dtype, int64_t x_ld,
@@ -270,7 +270,8 @@ int dlrm_split_weights(const dlrm_weight_planes *items, int32_t n, dlrm_stream_t
  * row-major (torch layout).  Any shape and leading dimension is accepted (K = 13, 479, ...);
  * operands whose rows start on 16-byte boundaries (pointer 16-byte aligned, leading dimension
  * a multiple of 4 floats) are read with 16-byte loads; others too, but for the operand's last row and a partial last
- * reduction step, which take 4-byte loads (DLRM_GEMM_F32_MFMA: 4-byte loads throughout).  Of an operand on other
+ * reduction step, which take 4-byte loads (DLRM_GEMM_F32_MFMA: 4-byte loads throughout), as do operands whose rows are so
+ * far apart that a tile of them spans 2^32 bytes (8.46 million floats from row to row and more).  Of an operand on other
  * boundaries nothing behind the last row's last element is read.  A leading dimension is a
  * promise that every row, the last one included, is readable up to it: when x_ld and w_ld both reach K rounded
  * up to 32, the columns between K and that bound are loaded too (and discarded; they need not be zero).
@@ -323,8 +324,9 @@ int dlrm_absmax(const float *d_x, int64_t rows, int32_t cols, int64_t ld, float 
  *                    x8 (d_codes != NULL) is the 8-bit checkpoint of x in
  *                    d_x's place: the product with the values it stands for.
  *                    They are exact bf16 numbers, so dz alone is cut into its
- *                    three bf16 pieces and the product has float32 accuracy
- *                    from three bf16 terms; gemm_mode has no say in it.
+ *                    three bf16 pieces: three terms per product, each exact,
+ *                    added in float32 (three additions where a float32
+ *                    product has one); gemm_mode has no say in it.
  *                    Leading dimensions of dz and x8 up to 2^24.
  */
 typedef struct dlrm_linear_bwd {
