@@ -1863,7 +1863,7 @@ static int launch_f16p(GemmParams p, const dlrm_weight_planes *wp, bool transpos
     return DLRM_OK;
 }
 // Largest batch: the kernels number rows with ints, and a range's nominal end or the next row of a thread that strides over the
-// batch lies up to 2^18 rows behind the last one.
+// batch lies up to 2^17 rows behind the last one.
 constexpr int64_t kMostRows = (1ll << 31) - (1 << 20);
 
 // rows of an operand start on 16-byte boundaries
